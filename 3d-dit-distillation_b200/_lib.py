@@ -63,6 +63,18 @@ SIGNATURES = {
     "vdit_linear": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp]),
     "vdit_linear_qkv_rope3d": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _vp,
                                               _vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _vp]),
+    "vdit_mxfp4_scale_bytes": (_c_sz, [_c_i64, _c_i32]),
+    "vdit_mxfp4_quantize": (ctypes.c_int, [_vp, _c_i32, _c_i64, _c_i64, _c_i32, _vp, _vp, _vp]),
+    "vdit_mxfp4_dequantize": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i32, _vp, _c_i32, _c_i64, _vp]),
+    "vdit_linear_mxfp4": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp]),
+    "vdit_kv_cache_write": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i32,
+                                           _c_i32, _c_i32, _c_i32, _vp]),
+    "vdit_kv_cache_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp, _c_i64, _vp,
+                                          _c_i64, _vp, _c_i64, _c_i32, _vp]),
+    "vdit_attention_1q_cached_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "vdit_attention_1q_cached": (ctypes.c_int, [_vp, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32,
+                                                _c_i32, _vp, _c_i64, _c_i32, _vp, _c_i32, _c_i32, _c_f32, _vp, _c_i64,
+                                                _vp, _c_sz, _vp]),
     "vdit_gather_rows_f32": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i32, _vp, _vp]),
     "vdit_cfg_reuse_workspace_bytes": (_c_sz, []),
     "vdit_cfg_reuse_euler": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_i32,

@@ -474,6 +474,9 @@ int pick_bn(int64_t m, int n) {
 
 }  // namespace gemm
 
+int kvcache_error_word(int clear);   // error word of the key/value cache (kvcache.cu)
+
+// the error word of the linears and, with them, of the cache their keys and values go to
 int gemm_error_word(int clear) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_gemm_error, sizeof(int)) != cudaSuccess) return VDIT_ERR_LAUNCH;
@@ -481,7 +484,8 @@ int gemm_error_word(int clear) {
         int z = 0;
         if (cudaMemcpyToSymbol(g_gemm_error, &z, sizeof(int)) != cudaSuccess) return VDIT_ERR_LAUNCH;
     }
-    return v;
+    const int c = kvcache_error_word(clear);
+    return v != 0 ? v : c;
 }
 
 }  // namespace vdit

@@ -1,0 +1,145 @@
+// Microscaled (MX) number formats: blocks of 32 consecutive elements of a row share one
+// power-of-two scale byte s (ue8m0: 2^(s - 127), 255 = NaN), elements are e2m1 (4 bits,
+// +-{0, .5, 1, 1.5, 2, 3, 4, 6}) or e4m3 (8 bits, up to 448).
+//
+// Quantising a block x: s - 127 = floor(log2(max|x|)) - emax, emax the exponent of the element
+// type's largest value (2 for e2m1, 8 for e4m3), no lower than -127; element = x * 2^(127 - s)
+// rounded to the nearest element value (ties to even, no further than the largest).  The scaling
+// is exact, so the one rounding is the element's.  A block with a NaN or an infinity, which
+// neither the 4-bit type nor the scale rule can hold, gets s = 255 and reads back as NaN.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace vdit {
+namespace mx {
+
+constexpr int kBlock = 32;
+
+// element types of the matrices that are quantised or read back (vdit.h VDIT_BF16 ...)
+template <int T> struct Elem;
+template <> struct Elem<VDIT_BF16> { using type = __nv_bfloat16; };
+template <> struct Elem<VDIT_F16> { using type = __half; };
+template <> struct Elem<VDIT_F32> { using type = float; };
+
+// 8 consecutive elements as fp32 (16-byte loads)
+__device__ __forceinline__ void load8_f32(const __nv_bfloat16* p, float* f) { load8_nc(p, f); }
+__device__ __forceinline__ void load8_f32(const __half* p, float* f) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(h[i]);
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+    }
+}
+__device__ __forceinline__ void load8_f32(const float* p, float* f) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void store8_f32(__nv_bfloat16* p, const float* f) { store8(p, f); }
+__device__ __forceinline__ void store8_f32(__half* p, const float* f) {
+    uint4 u;
+    __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = u;
+}
+__device__ __forceinline__ void store8_f32(float* p, const float* f) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+// max |f[i]| as fp32 bits: as integers the magnitudes order like the numbers, with the
+// infinity above every finite value and the NaNs above the infinity, so nothing is dropped
+__device__ __forceinline__ uint32_t amax8(const float* f) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+    return m;
+}
+
+// the scale byte of a block from its max |x| (fp32 bits).  The exponent field of a subnormal is
+// 0: below 2^-126 every block has the smallest scale.
+template <int BITS>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+    constexpr int emax = BITS == 4 ? 2 : 8;
+    const int e = (int)(amax >> 23);
+    return e == 255 ? 255u : (uint32_t)max(e - emax, 0);
+}
+
+// 2^(s - 127); s = 0 is the subnormal 2^-127, s = 255 a NaN
+__device__ __forceinline__ float scale_value(uint32_t s) {
+    return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fffffffu : s << 23);
+}
+// 2^(127 - s) for a scale of scale_byte (s <= 252), 0 for a NaN block (all its codes 0)
+__device__ __forceinline__ float scale_inverse(uint32_t s) {
+    return s == 255 ? 0.f : __uint_as_float((254u - s) << 23);
+}
+
+// 8 elements (already scaled) to codes: BITS bytes, element 0 in the lowest bits
+__device__ __forceinline__ uint32_t encode8_e2m1(const float* f) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r)
+        : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+    return r;
+}
+__device__ __forceinline__ uint2 encode8_e4m3(const float* f) {
+    uint2 r;
+    asm("{\n\t.reg .b16 h0, h1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h0, %3, %2;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h1, %5, %4;\n\t"
+        "mov.b32 %0, {h0, h1};\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h0, %7, %6;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h1, %9, %8;\n\t"
+        "mov.b32 %1, {h0, h1};\n\t}"
+        : "=r"(r.x), "=r"(r.y)
+        : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+    return r;
+}
+
+// codes to f16 pairs (every element value is an f16 value)
+__device__ __forceinline__ void decode8_e2m1(uint32_t c, __half2* h) {
+    uint32_t r[4];
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+        : "r"(c));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2*>(&r[i]);
+}
+__device__ __forceinline__ void decode4_e4m3(uint32_t c, __half2* h) {
+    uint32_t r[2];
+    asm("{\n\t.reg .b16 h0, h1;\n\t"
+        "mov.b32 {h0, h1}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, h0;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h1;\n\t}"
+        : "=r"(r[0]), "=r"(r[1])
+        : "r"(c));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) h[i] = *reinterpret_cast<__half2*>(&r[i]);
+}
+
+// The scales of a quantised matrix [rows, cols] are held in the order the block-scaled MMA
+// takes them from shared memory: 128 rows x 4 scales (128 columns) make one 512-byte block,
+// scale j of row r at (r % 32) * 16 + (r / 32) * 4 + j; the blocks of 128 rows follow one
+// another along the columns.  Rows and scales past the matrix are 0.
+__host__ __device__ constexpr int64_t scale_row_blocks(int64_t rows) { return (rows + 127) / 128; }
+__host__ __device__ constexpr int scale_col_groups(int cols) { return (cols + 127) / 128; }
+
+}  // namespace mx
+}  // namespace vdit

@@ -11,6 +11,9 @@ Reference names kept: ``precompute_rope_3d_table``, ``precompute_rope_2d_cond``,
 ``fast_swiglu_from_packed``, ``fast_out_modulate_unpatchify``,
 ``flash_varlen_qkvpacked_already_sorted``, ``flash_cross_attn``,
 ``flash_cond_self_attn``.
+
+The low-bit operators beside them (``quantize_mxfp4``, ``linear_mxfp4``, ``MxKvCache``,
+``attention_1q_cached`` and the rest) are this package's own, from ``microscaled``.
 """
 from __future__ import annotations
 
@@ -21,6 +24,8 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from ._lib import check, lib, ptr, stream_of
+from .microscaled import (MxKvCache, Mxfp4Tensor, attention_1q_cached, dequantize_mxfp4, kv_cache_read,  # noqa: F401
+                          kv_cache_write, linear_mxfp4, quantize_mxfp4)
 
 BF16 = torch.bfloat16
 

@@ -29,10 +29,15 @@ typedef void* vdit_stream_t;
 #define VDIT_ERR_ARG (-1)          /* bad shape / size / null pointer        */
 #define VDIT_ERR_ALIGN (-2)        /* pointer or stride not 16-byte aligned  */
 #define VDIT_ERR_LAUNCH (-3)       /* CUDA launch error                      */
-#define VDIT_ERR_UNSUPPORTED (-4)  /* head_dim / width not supported         */
+#define VDIT_ERR_UNSUPPORTED (-4)  /* head_dim, width or size not supported  */
 #define VDIT_ERR_WORKSPACE (-5)    /* workspace too small                    */
 #define VDIT_ERR_DRIVER (-6)       /* driver entry point (tensor maps) failed */
 #define VDIT_ERR_TOO_LARGE (-7)    /* beyond the fixed scratch of a no-alloc entry point */
+
+/* element types of dense matrices, for the entry points that take more than bf16 */
+#define VDIT_BF16 0
+#define VDIT_F16 1
+#define VDIT_F32 2
 
 /* ------------------------------------------------------------------ runtime */
 const char* vdit_version(void);
@@ -311,6 +316,72 @@ int vdit_linear_qkv_rope3d(const void* a, int64_t lda, const void* w, int64_t ld
                            const float* q_scale, const float* k_scale, const float* cos_t, const float* sin_t,
                            int32_t res, const int32_t* coords, const int64_t* dst_rows, void* out, int64_t ldo,
                            int64_t m, int32_t heads, int32_t head_dim, int32_t k, vdit_stream_t stream);
+
+/* ------------------------------------------------------------------ microscaled operands */
+/* Microscaled (MX) formats: 32 consecutive elements of a row share a scale byte s = 2^(s - 127)
+ * (255: NaN); elements are e2m1 (4 bits, two a byte, the even column in the low half) or e4m3
+ * (8 bits).  A block's scale is floor(log2(max |x|)) less the exponent of the element type's
+ * largest value (2 or 8), no lower than 2^-127; x / scale is rounded to the nearest element value,
+ * ties to even, no further than the largest (6 or 448).  A block with a NaN or an infinity gets
+ * scale 255 and reads back as NaN.  No counterpart in the reference, which computes in bf16.
+ *
+ * A quantised matrix [rows, cols] (cols a multiple of 32) is two 16-byte aligned buffers: codes,
+ * rows * cols / 2 bytes, and scales, vdit_mxfp4_scale_bytes(rows, cols) bytes in the order the
+ * block-scaled MMA reads them (blocks of 128 rows x 4 scales; scale j of row r of a block at byte
+ * (r % 32) * 16 + (r / 32) * 4 + j, blocks along the columns first; zero past the matrix).
+ *
+ * vdit_mxfp4_quantize writes both from x [rows, ldx] of x_type (VDIT_BF16, VDIT_F16, VDIT_F32);
+ * vdit_mxfp4_dequantize writes the values they stand for to out [rows, ldo] of out_type.  Dense
+ * rows start on 16-byte boundaries. */
+size_t vdit_mxfp4_scale_bytes(int64_t rows, int32_t cols);
+int vdit_mxfp4_quantize(const void* x, int32_t x_type, int64_t ldx, int64_t rows, int32_t cols, void* codes,
+                        void* scales, vdit_stream_t stream);
+int vdit_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int32_t cols, void* out,
+                          int32_t out_type, int64_t ldo, vdit_stream_t stream);
+
+/* out[m,n] = bf16(sum_k a[m,k] w[n,k] + bias[n]) of two quantised matrices a [m,k] and w [n,k]
+ * with fp32 accumulation: vdit_linear on 4-bit operands.  bias bf16 [n] or NULL, out bf16
+ * [m,ldo]; k a multiple of 32, n and ldo of 8, pointers 16-byte aligned. */
+int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
+                      const void* bias, void* out, int64_t ldo, int64_t m, int32_t n, int32_t k,
+                      vdit_stream_t stream);
+
+/* ------------------------------------------------------------------ key/value cache */
+/* A paged cache of keys and values in a microscaled format, bits 8 (e4m3) or 4 (e2m1).  Slot
+ * page * page_size + offset holds one row of heads * head_dim channels: kc and vc are
+ * [pages, heads, page_size, head_dim * bits / 8] bytes, k_scales and v_scales
+ * [pages, heads, page_size, head_dim / 32] bytes.  page_size is a power of two up to 1024;
+ * head_dim 32, 64, 96 or 128; kc, vc 16-byte aligned.
+ *
+ * write: rows k, v bf16 [n, ldk], [n, ldv] are quantised into slots[n]; a negative slot is
+ * skipped, and no slot may appear twice among the others.  read: the rows the slots stand for, bf16
+ * or fp32; a negative slot gives zeros.  A slot past the cache is left out (read: zeros) and
+ * recorded in the device error word. */
+int vdit_kv_cache_write(const void* k, int64_t ldk, const void* v, int64_t ldv, const int64_t* slots, int64_t n,
+                        void* kc, void* vc, void* k_scales, void* v_scales, int64_t pages, int32_t page_size,
+                        int32_t heads, int32_t head_dim, int32_t bits, vdit_stream_t stream);
+int vdit_kv_cache_read(const void* kc, const void* vc, const void* k_scales, const void* v_scales, int64_t pages,
+                       int32_t page_size, int32_t heads, int32_t head_dim, int32_t bits, const int64_t* slots,
+                       int64_t n, void* k, int64_t ldk, void* v, int64_t ldv, int32_t out_type,
+                       vdit_stream_t stream);
+
+/* One query per sequence and head over cached keys: vdit_attention_1q for a batch, reading the
+ * cache.  Sequence b attends to its first lengths[b] (int32) keys, key i in page
+ * page_table[b * ld_table + i / page_size] (int32) at offset i % page_size; entries past its
+ * length are not read (ld_table 0: every sequence has the same pages).  No keys give zeros.  q bf16 [batch, ldq] and out bf16 [batch, ldo] hold
+ * heads * head_dim channels a row; query head h reads key head h / (heads / kv_heads).  A page
+ * outside the cache is left out and a length outside [0, max_pages * page_size] is clipped to it,
+ * both recorded in the device error word.  Partial states of split key ranges go to the
+ * caller's workspace (of vdit_attention_1q_cached_workspace_bytes bytes, 16-byte aligned; may be
+ * 0). */
+size_t vdit_attention_1q_cached_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                                int32_t max_pages, int32_t page_size);
+int vdit_attention_1q_cached(const void* q, int64_t ldq, const void* kc, const void* vc, const void* k_scales,
+                             const void* v_scales, int64_t pages, int32_t page_size, int32_t kv_heads,
+                             int32_t head_dim, int32_t bits, const int32_t* page_table, int64_t ld_table,
+                             int32_t max_pages, const int32_t* lengths, int32_t batch, int32_t heads,
+                             float softmax_scale, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                             vdit_stream_t stream);
 
 /* ------------------------------------------------------------------ sampler glue */
 /* dst[j,:] = src[idx[j],:] for fp32 rows of width c (noise[perm], lib/fast_flow.py:2576). */

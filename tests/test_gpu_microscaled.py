@@ -1,0 +1,445 @@
+"""GPU tests of the low-bit operators against their 64-bit restatement (oracle/microscaled.py).
+
+Quantised values are compared exactly: the scaling is a power of two and the one rounding is the
+element's, so there is nothing to be near to.  Products and attention come with bounds counted
+from the arithmetic, written at each helper."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from vdit import _lib
+from vdit import fast_kernels as fk
+
+from oracle import microscaled as mxo
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    yield
+    assert _lib.device_error(clear=True) == 0
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def host(t):
+    return t.detach().cpu().double().numpy()
+
+
+def same(a, b):
+    """Equal values, NaN where the other has NaN."""
+    return np.array_equal(a, b, equal_nan=True)
+
+
+def rows(g, m, k, dtype=BF16, spread=3.0):
+    """Normal rows whose blocks differ in size by powers of two."""
+    x = torch.randn(m, k, generator=g, device=DEV)
+    s = torch.exp2(torch.randn(m, k // 32, generator=g, device=DEV) * spread).repeat_interleave(32, 1)
+    return (x * s).to(dtype)
+
+
+# ----------------------------------------------------------------------------- 4-bit matrices
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 32), (1, 1536), (2, 96), (33, 128), (127, 160), (129, 288), (300, 2080)])
+def test_quantized_values_are_exact(m, k, dtype):
+    x = rows(gen(m * 10007 + k), m, k, dtype)
+    q = fk.quantize_mxfp4(x)
+    want = mxo.values(host(x), 4)
+    assert same(host(fk.dequantize_mxfp4(q, torch.float32)), want)
+    assert same(host(fk.dequantize_mxfp4(q)), want)
+    with np.errstate(over="ignore"):
+        assert same(host(fk.dequantize_mxfp4(q, torch.float16)), want.astype(np.float16).astype(np.float64))
+    code, neg, scale = mxo.quantize(host(x), 4)
+    c = q.codes.cpu().numpy()
+    got = np.stack([c & 15, c >> 4], -1).reshape(m, k)
+    assert np.array_equal(got & 7, code) and np.array_equal((got >> 3).astype(bool), neg)
+    # the scales in the block-scaled MMA's order, zero past the matrix
+    s = q.scales.cpu().numpy().reshape(-(-m // 128), -(-k // 128), 32, 4, 4).transpose(0, 3, 2, 1, 4)
+    s = s.reshape(-(-m // 128) * 128, -1)
+    assert np.array_equal(s[:m, :k // 32], scale)
+    assert not s[m:].any() and not s[:, k // 32:].any()
+
+
+def test_quantize_special_blocks():
+    """Zeros, subnormals, the largest numbers, halves between elements, NaN and infinities."""
+    big = torch.finfo(torch.float32).max
+    grid = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.99, 0.2499999, 0.2500001, -0.25, -5, -7, -0.0])
+    x = torch.zeros(12, 64)
+    x[1, :32] = torch.arange(32) * 2.0 ** -149                       # subnormal fp32
+    x[2, :32] = 2.0 ** -126 * torch.linspace(0, 1, 32)
+    x[3, :32] = big * torch.linspace(-1, 1, 32)
+    x[4, :16], x[4, 16:32] = grid, -grid
+    x[5, :32] = torch.cat([grid, -grid]) * 2.0 ** 100
+    x[6, 5], x[6, 40] = math.nan, 3.0
+    x[7, 31], x[7, 33] = math.inf, -1.0
+    x[8, 0], x[8, 63] = -math.inf, math.nan
+    x[9] = 1e-3
+    x[10, ::2] = -0.0
+    x[11, :32] = 2.0 ** torch.arange(-16, 16).float()
+    got = host(fk.dequantize_mxfp4(fk.quantize_mxfp4(x.to(DEV)), torch.float32))
+    want = mxo.values(x.double().numpy(), 4)
+    assert same(got, want)
+    assert np.isnan(got[6, :32]).all() and (got[6, 32:] != 0).sum() == 1
+    assert not got[0].any()
+
+
+def test_quantize_strided_rows_and_empty():
+    g = gen(5)
+    wide = rows(g, 70, 512)
+    for v in (wide[:, 128:288], wide[::3, 64:96], wide[5:6, 8:40], wide[7:8].expand(1, 512)):
+        q = fk.quantize_mxfp4(v)
+        assert same(host(fk.dequantize_mxfp4(q)), mxo.values(host(v), 4))
+    with pytest.raises(RuntimeError, match="aligned"):
+        fk.quantize_mxfp4(wide[:, 4:36])
+    with pytest.raises(RuntimeError, match="aligned"):
+        fk.quantize_mxfp4(torch.zeros(4, 36, dtype=BF16, device=DEV)[:, :32])
+    e = fk.quantize_mxfp4(wide[:0])
+    assert e.shape == (0, 512) and fk.dequantize_mxfp4(e).shape == (0, 512)
+    assert fk.linear_mxfp4(e, fk.quantize_mxfp4(wide[:8])).shape == (0, 8)
+
+
+# ----------------------------------------------------------------------------- linear
+
+def check_linear(got, x, w, bias):
+    """fp32 sums of k exact products in some order, each addition off by at most 2^-23 of the sum
+    of magnitudes (a rounded one by 2^-24; the matrix units may truncate), then one rounding to
+    bf16 (2^-8 of the value)."""
+    want, mag = mxo.linear(host(x), host(w), None if bias is None else host(bias))
+    acc = (x.shape[1] + 2) * 2.0 ** -23 * mag
+    err = np.abs(host(got) - want)
+    assert np.isfinite(host(got)).all()
+    assert (err <= acc + 2.0 ** -8 * (np.abs(want) + acc) + 1e-38).all(), (err - acc).max()
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (1, 8, 32), (1, 1536, 1536), (1, 200, 3840), (2, 264, 96), (5, 1000, 160), (7, 64, 2080), (8, 136, 352),
+    (9, 136, 352), (16, 1536, 256), (17, 72, 64), (33, 200, 1280), (127, 128, 128), (128, 192, 256), (129, 200, 288),
+    (250, 1536, 1536), (300, 392, 1280), (1000, 776, 3840), (257, 7680, 160), (4101, 1536, 512), (20000, 384, 64)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_linear_matches_64_bits(m, n, k, with_bias):
+    g = gen(m * 131 + n * 17 + k)
+    x, w = rows(g, m, k, spread=1.0), rows(g, n, k, spread=1.0)
+    bias = torch.randn(n, generator=g, device=DEV).to(BF16) if with_bias else None
+    wq = fk.quantize_mxfp4(w)
+    got = fk.linear_mxfp4(x, wq, bias)
+    assert got.shape == (m, n) and got.dtype == BF16
+    check_linear(got, x, w, bias)
+    # quantised by the caller, or again: the same operands in the same order
+    xq = fk.quantize_mxfp4(x)
+    a = fk.linear_mxfp4(xq, wq, bias)
+    check_linear(a, x, w, bias)
+    assert torch.equal(a, fk.linear_mxfp4(xq, wq, bias)) and torch.equal(got, fk.linear_mxfp4(x, wq, bias))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("m", [1, 6, 140])
+def test_linear_takes_other_types(m, dtype):
+    g = gen(m)
+    x, w = rows(g, m, 320, dtype, spread=1.0), rows(g, 208, 320, dtype, spread=1.0)
+    check_linear(fk.linear_mxfp4(x, fk.quantize_mxfp4(w)), x, w, None)
+
+
+@pytest.mark.parametrize("m", [1, 4, 8, 40, 200])
+def test_linear_spreads_nan_over_its_row_and_column_only(m):
+    g = gen(90 + m)
+    x, w = rows(g, m, 256, spread=1.0), rows(g, 136, 256, spread=1.0)
+    x[m // 2, 70], w[11, 200], w[100, 3] = math.nan, math.inf, math.nan
+    got = host(fk.linear_mxfp4(x, fk.quantize_mxfp4(w)))
+    bad = np.zeros((m, 136), dtype=bool)
+    bad[m // 2], bad[:, 11], bad[:, 100] = True, True, True
+    assert np.array_equal(np.isnan(got), bad)
+
+
+@pytest.mark.parametrize("m", [3, 150])
+def test_linear_writes_its_part_of_out_only(m):
+    g = gen(m)
+    x, w = rows(g, m, 128, spread=1.0), rows(g, 72, 128, spread=1.0)
+    wq = fk.quantize_mxfp4(w)
+    out = torch.full((m + 3, 160), 7.0, dtype=BF16, device=DEV)
+    view = out[1:, 16:]
+    assert fk.linear_mxfp4(x, wq, out=view) is view
+    assert torch.equal(out[1:m + 1, 16:88], fk.linear_mxfp4(x, wq))
+    out[1:m + 1, 16:88] = 7
+    assert (out == 7).all()
+
+
+@pytest.mark.parametrize("m", [2, 130])
+def test_linear_over_the_range_of_scales(m):
+    """Blocks near both ends of the scale's range: large times small comes out in between."""
+    x = torch.full((m, 96), 2.0 ** 100, dtype=BF16, device=DEV)
+    w = torch.full((8, 96), -1.5 * 2.0 ** -98, dtype=BF16, device=DEV)
+    x[:, 32:64], w[:, 64:] = 2.0 ** -120, 0
+    want = -1.5 * 4 * 32                                     # the second block adds nothing that bf16 holds
+    assert (fk.linear_mxfp4(x, fk.quantize_mxfp4(w)).float() == want).all()
+
+
+# ----------------------------------------------------------------------------- cache
+
+def filled(g, pages, page, heads, hd, bits):
+    """A cache whose every slot is written, and the rows that went in."""
+    c = fk.MxKvCache(pages, page, heads, hd, bits=bits, device=DEV)
+    k, v = (torch.randn(c.slots, c.width, generator=g, device=DEV).to(BF16) for _ in range(2))
+    fk.kv_cache_write(c, k, v, torch.arange(c.slots, device=DEV))
+    return c, k, v
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("heads,hd,page", [(1, 32, 1), (3, 64, 16), (5, 96, 32), (12, 128, 64), (2, 128, 1024)])
+def test_cache_holds_what_was_written(heads, hd, page, bits):
+    g = gen(heads * 1000 + hd + page + bits)
+    c = fk.MxKvCache(3, page, heads, hd, bits=bits, device=DEV)
+    n = max(1, c.slots // 2)
+    both = rows(g, n, 2 * c.width)                            # keys and values as halves of one matrix
+    k, v = both[:, :c.width], both[:, c.width:]
+    slots = torch.randperm(c.slots, generator=g, device=DEV)[:n]
+    skip = torch.arange(n, device=DEV) % 5 == 3
+    fk.kv_cache_write(c, k, v, torch.where(skip, -1 - slots, slots))
+    want = [np.zeros((c.slots, c.width)) for _ in range(2)]
+    at = slots[~skip].cpu().numpy()
+    for w, t in zip(want, (k, v)):
+        w[at] = mxo.values(host(t), bits)[~skip.cpu().numpy()]
+    back = torch.randperm(c.slots, generator=g, device=DEV)
+    for dtype in (BF16, torch.float32):
+        got = fk.kv_cache_read(c, back, dtype)
+        for a, b in zip(got, want):
+            assert a.dtype == dtype and same(host(a), b[back.cpu().numpy()])   # untouched slots are zeros still
+    back[::2] = -7
+    for a in fk.kv_cache_read(c, back):
+        assert not a[::2].any()
+    none = torch.empty(0, dtype=torch.int64, device=DEV)
+    fk.kv_cache_write(c, k[:0], v[:0], none)
+    assert fk.kv_cache_read(c, none)[0].shape == (0, c.width)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_cache_special_blocks(bits):
+    c = fk.MxKvCache(1, 4, 1, 64, bits=bits, device=DEV)
+    x = torch.zeros(4, 64)
+    x[0, 3], x[0, 40] = math.nan, 1.0
+    x[1, 33], x[2, 0] = -math.inf, 2.0 ** -130
+    x[3] = torch.cat([torch.linspace(440, 511, 32), torch.linspace(0.0, 0.05, 32)])
+    x = x.to(BF16)
+    fk.kv_cache_write(c, x.to(DEV), -x.to(DEV), torch.arange(4, device=DEV))
+    k, v = fk.kv_cache_read(c, torch.arange(4, device=DEV), torch.float32)
+    assert same(host(k), mxo.values(host(x), bits)) and same(host(v), mxo.values(host(-x), bits))
+
+
+def test_slots_outside_the_cache_are_left_out_and_recorded():
+    g = gen(1)
+    c, k, v = filled(g, 2, 16, 2, 32, 8)
+    before = [t.clone() for t in (c.k, c.v, c.k_scales, c.v_scales)]
+    slots = torch.tensor([32, 1 << 40, -1], device=DEV)
+    fk.kv_cache_write(c, k[:3], v[:3], slots)
+    assert _lib.device_error(clear=True) == 0x4B56
+    assert all(torch.equal(a, b) for a, b in zip(before, (c.k, c.v, c.k_scales, c.v_scales)))
+    a, b = fk.kv_cache_read(c, torch.tensor([32, 3], device=DEV))
+    assert _lib.device_error(clear=True) == 0x4B56
+    assert not a[0].any() and not b[0].any() and same(host(a[1]), mxo.values(host(k[3:4]), 8)[0])
+
+
+# ----------------------------------------------------------------------------- attention over the cache
+
+def check_attend(got, q, c, k, v, table, lengths, bits, scale=None):
+    """Scores are fp32 sums of head_dim products (each addition off by 2^-24 of the magnitudes'
+    sum, the query's scaling by another), so a weight is off by e^d - 1 with d that error in
+    natural units, and by 2^-21 of itself through two base-2 exponentials (2 ulp each and the
+    rescaling); sums over n keys and their quotient add (n + 8) 2^-24.  The error of the weights
+    counts twice, above and below the fraction.  Then one rounding to bf16."""
+    hk, hd, page = c.kv_heads, c.head_dim, c.page_size
+    h = q.shape[1] // hd
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    kv, vv = (mxo.values(host(t), bits).reshape(c.slots, hk, hd) for t in (k, v))
+    t, out = table.cpu().numpy(), host(got)
+    for b, n in enumerate(lengths):
+        at = np.arange(n)
+        r = t[b][at // page].astype(np.int64) * page + at % page if n else at
+        want, mag, unit = mxo.attend(host(q[b]).reshape(h, hd), kv[r], vv[r], scale)
+        d = (hd + 4) * 2.0 ** -24 * unit
+        rel = 2 * (np.expm1(d) + 2.0 ** -21) + (n + 8) * 2.0 ** -24
+        e = rel[:, None] * mag
+        err = np.abs(out[b].reshape(h, hd) - want)
+        assert (err <= e + 2.0 ** -8 * (np.abs(want) + e)).all(), (b, n, err.max())
+
+
+def paged(g, c, lengths, spare=0):
+    """A table of pages in no order, -1 past each sequence's last page."""
+    need = [-(-n // c.page_size) for n in lengths]
+    order = torch.randperm(c.pages, generator=g, device=DEV).to(torch.int32)
+    assert sum(need) <= c.pages
+    t = torch.full((len(lengths), max(max(need), 1) + spare), -1, dtype=torch.int32, device=DEV)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = order[at:at + n]
+        at += n
+    return t
+
+
+def i32(vals):
+    return torch.tensor(vals, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hk,grp,hd,page", [(2, 1, 32, 1), (3, 2, 64, 16), (5, 1, 96, 32), (12, 1, 128, 64),
+                                            (2, 3, 128, 16), (1, 4, 96, 128), (2, 5, 64, 32), (1, 9, 128, 16),
+                                            (4, 4, 96, 16)])
+def test_attention_over_ragged_pages(hk, grp, hd, page, bits):
+    g = gen(hk * 100 + grp * 10 + hd + page + bits)
+    lengths = [1, 0, page, page + 1, 3 * page - 1, 130, 517]
+    c, k, v = filled(g, sum(-(-n // page) for n in lengths) + 2, page, hk, hd, bits)
+    q = (torch.randn(len(lengths), hk * grp * hd, generator=g, device=DEV) * 2).to(BF16)
+    t = paged(g, c, lengths, spare=2)
+    got = fk.attention_1q_cached(q, c, t, i32(lengths))
+    assert not got[1].any()
+    check_attend(got, q, c, k, v, t, lengths, bits)
+    assert torch.equal(got, fk.attention_1q_cached(q, c, t, i32(lengths)))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("batch,n,hk,grp,hd,page", [(1, 4101, 12, 1, 128, 64), (1, 20000, 2, 1, 96, 128),
+                                                    (40, 300, 3, 2, 64, 16), (300, 33, 2, 1, 32, 32)])
+def test_attention_splits_and_batches(batch, n, hk, grp, hd, page, bits):
+    g = gen(n + batch)
+    lengths = [max(0, n - (i * 37) % (n + 1)) for i in range(batch)]
+    c, k, v = filled(g, sum(-(-m // page) for m in lengths) + 1, page, hk, hd, bits)
+    wide = torch.randn(batch, hk * grp * hd + 64, generator=g, device=DEV).to(BF16)
+    q = wide[:, 64:]                                          # a strided view
+    t = paged(g, c, lengths)
+    check_attend(fk.attention_1q_cached(q, c, t, i32(lengths)), q, c, k, v, t, lengths, bits)
+
+
+def test_attention_peaked_scores_and_scale():
+    """Scores hundreds apart, growing along the keys (the running maximum moves all the time) and
+    falling; a given softmax scale, also a negative one."""
+    g = gen(3)
+    c = fk.MxKvCache(40, 16, 1, 64, bits=8, device=DEV)
+    ramp = torch.linspace(-4, 4, c.slots, device=DEV)[:, None]
+    v = torch.randn(c.slots, 64, generator=g, device=DEV).to(BF16)
+    k = (ramp * torch.ones(1, 64, device=DEV)).to(BF16)
+    fk.kv_cache_write(c, k, v, torch.arange(c.slots, device=DEV))
+    q = torch.ones(1, 64, device=DEV, dtype=BF16) * 4
+    t = torch.arange(40, dtype=torch.int32, device=DEV)[None]
+    for scale in (None, 1.0, -1.0, 0.0):
+        for table in (t, t.flip(1)):
+            got = fk.attention_1q_cached(q, c, table.contiguous(), i32([c.slots]), scale)
+            check_attend(got, q, c, k, v, table, [c.slots], 8, scale)
+
+
+def test_attention_nan_stays_in_its_sequence_and_head():
+    g = gen(4)
+    c, k, v = filled(g, 8, 16, 2, 64, 8)
+    k[20, 70], v[100, 3] = math.nan, math.inf                 # head 1 of page 1, head 0 of page 6
+    fk.kv_cache_write(c, k, v, torch.arange(c.slots, device=DEV))
+    q = torch.randn(4, 128, generator=g, device=DEV).to(BF16)
+    t = i32([[0, 1], [2, 3], [6, 7], [1, 0]])
+    got = host(fk.attention_1q_cached(q, c, t, i32([32, 32, 32, 4]))).reshape(4, 2, 64)
+    bad = np.isnan(got)
+    assert bad[0, 1].all() and not bad[0, 0].any() and not bad[1].any()
+    assert bad[2, 0, :32].all() and not bad[2, 0, 32:].any() and not bad[2, 1].any()
+    assert not bad[3].any()                                   # the NaN lies past this length
+
+
+def test_attention_one_table_for_all_and_bad_pages():
+    g = gen(6)
+    c, k, v = filled(g, 6, 32, 3, 96, 4)
+    q = torch.randn(5, 3 * 96, generator=g, device=DEV).to(BF16)
+    shared = i32([[4, 1, 5]]).expand(5, 3)                    # row stride 0: one prefix for all
+    lengths = [96, 40, 1, 0, 64]
+    check_attend(fk.attention_1q_cached(q, c, shared, i32(lengths)), q, c, k, v, shared, lengths, 4)
+    # a page that is not there: its keys are left out; lengths past the table end with it
+    t = i32([[4, 6, 5], [4, -1, 5], [4, 1, 5], [4, 1, 5], [0, 2, 3]])
+    got = fk.attention_1q_cached(q, c, t, i32([96, 96, 1000, -3, 64]))
+    assert _lib.device_error(clear=True) == 0x4B56
+    two, three = i32([[4, 5]] * 5), i32([[4, 1, 5]] * 5)
+    check_attend(got[:2], q[:2], c, k, v, two, [64, 64], 4)
+    check_attend(got[2:3], q[2:3], c, k, v, three, [96], 4)
+    assert not got[3].any()
+
+
+# ----------------------------------------------------------------------------- together
+
+def test_a_served_block_step_by_step():
+    """What a server of one block's attention does: the K/V linear in 4 bits, its rows written into the
+    cache as they come, one query per sequence over them, the output linear; and the cached rows
+    read back for the many-query attention."""
+    g = gen(11)
+    heads, hd, page = 4, 64, 16
+    d = heads * hd
+    wkv, wo = (torch.randn(n, d, generator=g, device=DEV).to(BF16) * 0.05 for n in (2 * d, d))
+    qkv, qo = fk.quantize_mxfp4(wkv), fk.quantize_mxfp4(wo)
+    c = fk.MxKvCache(12, page, heads, hd, bits=8, device=DEV)
+    table = torch.randperm(12, generator=g, device=DEV).to(torch.int32).view(3, 4)
+    lengths = [0, 0, 0]
+    k_in, v_in = (torch.zeros(c.slots, d, dtype=BF16, device=DEV) for _ in range(2))
+    for step in range(3):
+        new = [17, 1, 20] if step == 0 else [1, 1, 1]
+        if step == 2:
+            new = [1, 0, 1]                                   # one sequence pauses
+        x = torch.randn(sum(new), d, generator=g, device=DEV).to(BF16)
+        kv = fk.linear_mxfp4(x, qkv)
+        at = [(b, lengths[b] + i) for b in range(3) for i in range(new[b])]
+        slots = torch.tensor([int(table[b, i // page]) * page + i % page for b, i in at], device=DEV)
+        fk.kv_cache_write(c, kv[:, :d], kv[:, d:], slots)
+        k_in[slots], v_in[slots] = kv[:, :d], kv[:, d:]
+        lengths = [a + b for a, b in zip(lengths, new)]
+        q = torch.randn(3, d, generator=g, device=DEV).to(BF16)
+        o = fk.attention_1q_cached(q, c, table, i32(lengths))
+        check_attend(o, q, c, k_in, v_in, table, lengths, 8)
+        y = fk.linear_mxfp4(o, qo)
+        check_linear(y, o, wo, None)
+    # the same sequence through the many-query attention, which takes bf16 rows
+    n = lengths[0]
+    r = torch.tensor([int(table[0, i // page]) * page + i % page for i in range(n)], device=DEV)
+    k, v = fk.kv_cache_read(c, r)
+    assert same(host(k), mxo.values(host(k_in[r]), 8)) and same(host(v), mxo.values(host(v_in[r]), 8))
+
+
+def test_captured_and_on_another_stream():
+    """One graph of the whole step replayed on new inputs, beside a second graph of the same calls
+    and eager calls on another stream: each has its own workspace."""
+    g = gen(12)
+    heads, hd, page, d = 3, 128, 16, 384
+    wq = fk.quantize_mxfp4(torch.randn(d, d, generator=g, device=DEV).to(BF16) * 0.05)
+
+    def step(s):
+        fk.kv_cache_write(s["c"], s["k"], s["v"], s["slots"])
+        o = fk.attention_1q_cached(s["q"], s["c"], s["t"], s["n"])
+        return o, fk.linear_mxfp4(o, wq), fk.kv_cache_read(s["c"], s["slots"])[0]
+
+    def state(seed):
+        gg = gen(seed)
+        s = {n: torch.randn(r, d, generator=gg, device=DEV).to(BF16) for n, r in (("k", 60), ("v", 60), ("q", 2))}
+        s["c"] = fk.MxKvCache(80, page, heads, hd, device=DEV)
+        s["slots"] = torch.randperm(60, generator=gg, device=DEV)
+        s["t"] = torch.arange(80, dtype=torch.int32, device=DEV).view(2, 40)
+        s["n"] = i32([60, 7])
+        return s
+
+    states, graphs = [state(1), state(2)], []
+    step(states[0])
+    for s in states:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(s)
+        graphs.append((graph, out))
+    side = torch.cuda.Stream()
+    for seed in (21, 22, 23):
+        fresh = [state(seed), state(seed + 100)]
+        for s, f in zip(states, fresh):
+            for n in ("k", "v", "q", "slots"):
+                s[n].copy_(f[n])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            want = [step(f) for f in fresh]
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, got), w in zip(graphs, want):
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
