@@ -474,7 +474,8 @@ int pick_bn(int64_t m, int n) {
 
 }  // namespace gemm
 
-int kvcache_error_word(int clear);   // error word of the key/value cache (kvcache.cu)
+int kvcache_error_word(int clear);    // error word of the key/value cache (kvcache.cu)
+int mxlinear_error_word(int clear);   // error word of the 4-bit linear (mxlinear.cu)
 
 // the error word of the linears and, with them, of the cache their keys and values go to
 int gemm_error_word(int clear) {
@@ -484,8 +485,9 @@ int gemm_error_word(int clear) {
         int z = 0;
         if (cudaMemcpyToSymbol(g_gemm_error, &z, sizeof(int)) != cudaSuccess) return VDIT_ERR_LAUNCH;
     }
-    const int c = kvcache_error_word(clear);
-    return v != 0 ? v : c;
+    for (int w : {mxlinear_error_word(clear), kvcache_error_word(clear)})
+        if (v == 0) v = w;
+    return v;
 }
 
 }  // namespace vdit

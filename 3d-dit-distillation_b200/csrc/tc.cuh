@@ -262,6 +262,45 @@ __host__ __device__ constexpr uint32_t make_idesc(int m, int n, bool b_mn_major)
            ((uint32_t)(m >> 4) << 24);
 }
 
+// ---------------------------------------------------------------- block-scaled 4-bit MMAs
+// instruction descriptor of kind::mxf4: f32 accumulate, e2m1 A/B (K-major), ue8m0 scales; sf picks
+// the scale bytes (0 or 2: the low or the high two of a TMEM word) of both operands
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int sf) {
+    return ((uint32_t)sf << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+           ((uint32_t)(m >> 7) << 27) | ((uint32_t)sf << 29);
+}
+
+// D (TMEM) += (A * its scales) (B * its scales), K = 64 (two blocks of 32 a row), issued by the
+// elected lane of a converged warp
+__device__ __forceinline__ void tc_mma_mxf4_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                  uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accum) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accum)
+        : "memory");
+}
+
+// 32 rows x 16 bytes of shared memory -> 4 TMEM columns of lanes 0..31, repeated in the other
+// three lane quarters; ordered before the MMAs the same lane issues after it
+__device__ __forceinline__ void tc_cp_scales_elect(uint32_t tmem, uint64_t desc) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}"
+        ::"r"(tmem), "l"(desc)
+        : "memory");
+}
+
+// untiled bulk copy (16-byte aligned, a multiple of 16 bytes) counted on an mbarrier of this CTA
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 // ---------------------------------------------------------------- CTA pairs (cta_group::2)
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
