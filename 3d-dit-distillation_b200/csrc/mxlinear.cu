@@ -1,22 +1,24 @@
 // Linear on 4-bit microscaled operands (mx.cuh) on the block-scaled tcgen05 MMA:
 //   out[m, n] = bf16( sum over blocks b of 2^(sa[m,b] + sw[n,b]) * sum_{j < 32} a[m,b,j] w[n,b,j] + bias[n] )
 //
-// A persistent CTA per SM walks 128 x BN output tiles.  A k-step is 256 elements (128 bytes) of
-// 128 rows of a and BN rows of w, and their scales.  Warp roles:
+// Persistent CTA pairs (clusters of two, cta_group::2) walk 256 x BN output tiles, or, for few
+// tiles, single CTAs 128 x BN ones.  A k-step is 256 elements (128 bytes) of 128 rows of a and of
+// the CTA's share of the BN rows of w, and their scales.  Warp roles in each CTA:
 //   warp 0      TMA producer: the codes as 128-byte-wide boxes (128-byte swizzle, K-major), the
-//               scales as untiled copies of the 512-byte blocks they are stored in, all of a
-//               k-step on one barrier of a ring
-//   warp 1      MMA issuer: copies the k-step's scales from shared memory to TMEM (tcgen05.cp; each
-//               ring stage has its own columns, free when the stage is), then up to four
-//               128 x BN x 64 MMAs into one of two TMEM accumulators
-//   warps 2..5  epilogue: bias, rounding and TMA stores of one accumulator while the MMAs of the
+//               scales in the 512-byte blocks they are stored in, into a ring; a pair's loads
+//               all complete on the even CTA's stage barrier
+//   warp 1      MMA issuer (even CTA): copies the k-step's scales from shared memory to the ring
+//               stage's TMEM columns (tcgen05.cp), then four 64-deep MMAs
+//   warps 2..9  epilogue: bias, rounding and TMA stores of one accumulator while the MMAs of the
 //               next tile fill the other
-// 192 columns is the widest tile whose two accumulators leave TMEM room for the scales (2 x 192 +
-// 4 stages x 24 of 512 columns); its tiles start on every other 64 rows of w, so an odd tile reads
-// its scales from two columns further on.
+// A k-step's MMAs take 512 clocks at the full rate, whatever its element type, so the issuer has to
+// get through a k-step's waits, copies and MMAs in less; the notes in its loop say what that took.
+// Two 256-column accumulators and 5 stages x 24 columns of scales do not fit TMEM's 512, so the
+// second accumulator starts 120 columns early and each tile's epilogue empties the shared columns
+// first, before the next tile's MMAs start.
 //
 // Every mbarrier wait is bounded; a wait that runs out records an error in g_mxlinear_error,
-// raises the CTA abort flag and the CTA skips to its teardown (TMEM always freed).
+// raises the CTA abort flag and the CTA skips to its teardown (cluster barrier, TMEM always freed).
 #include <string.h>
 
 #include <algorithm>
@@ -34,29 +36,29 @@ namespace {
 
 using namespace tc;
 
-constexpr int BM = 128;
+constexpr int BM = 128;                 // rows per CTA
 constexpr int BK = 256;                 // elements of a k-step: 128 bytes of codes
-constexpr int EPI_WARPS = 4;
+constexpr int EPI_WARPS = 8;             // two for each quarter of the 128 TMEM lanes
 constexpr int kThreads = (2 + EPI_WARPS) * 32;
 constexpr int kErr = 0x4D58;            // "MX": a bounded wait of the linear ran out
 constexpr int kScaleBlock = 512;        // 128 rows x 4 scales
 
-template <int BN>
+template <int CG, int BN>
 struct __align__(1024) Smem {
-    static constexpr int NBLK = BN == 192 ? 2 : 1;          // 128-row scale blocks a tile of w touches
-    static constexpr int NST = BN == 192 ? 4 : BN == 128 ? 5 : 6;
+    static constexpr int NBLK = BN > 128 ? 2 : 1;           // 128-row scale blocks a tile of w touches
+    static constexpr int NST = BN > 128 ? 5 : 6;
     uint8_t a[NST][BM * 128];
-    uint8_t w[NST][BN * 128];
-    uint8_t x[EPI_WARPS * 2 * 32 * 128];                    // two 32-row x 64-column boxes a warp
+    uint8_t w[NST][BN / CG * 128];                          // this CTA's share of the weight tile
+    uint8_t x[EPI_WARPS][32 * 128];                         // a 32-row x 64-column box a warp
     uint8_t sa[NST][2 * kScaleBlock];
-    uint8_t sw[NST][NBLK][2 * kScaleBlock];
-    uint64_t full[NST], empty[NST], acc_full[2], acc_empty[2];
+    uint8_t sw[NST][NBLK][2 * kScaleBlock];                 // the scales of the whole weight tile
+    float bias[EPI_WARPS][BN];
+    uint64_t full[NST], empty[NST], acc_full[2], acc_empty[2], shared_empty;
     uint32_t tmem_slot;
     int abort_flag;
 };
 
 struct Args {
-    const uint8_t *as, *ws;             // scales
     const __nv_bfloat16* bias;
     int64_t m;
     int n, k;
@@ -78,26 +80,54 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
                  : "memory");
 }
 
-template <int BN>
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (CG == 1) tma_load_2d(dst, map, x, y, bar);
+    else tma_load_2d_pair(dst, map, x, y, mapa_shared(bar, 0));
+}
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (CG == 1) tc_commit_elect(bar);
+    else tc_commit_pair_elect(bar, 0x3);
+}
+// One arrival on the MMA issuer's barrier (in the even CTA of a pair), after the thread's TMEM loads
+// have completed.  Nothing in memory is handed over, so the odd CTA's arrival is a relaxed one: a
+// release to the cluster took ~1000 clocks here, between a tile's last MMA and the next one's first.
+template <int CG>
+__device__ __forceinline__ void arrive_issuer(uint32_t bar, uint32_t rank) {
+    if (CG == 1 || rank == 0) mbar_arrive(bar);
+    else
+        asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa_shared(bar, 0)) : "memory");
+}
+
+template <int CG, int BN>
 __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_constant__ CUtensorMap tmA,
                                                              const __grid_constant__ CUtensorMap tmW,
+                                                             const __grid_constant__ CUtensorMap tmSA,
+                                                             const __grid_constant__ CUtensorMap tmSW,
                                                              const __grid_constant__ CUtensorMap tmO,
                                                              const __grid_constant__ Args p) {
     extern __shared__ uint8_t raw[];
-    using SM = Smem<BN>;
-    constexpr int NST = SM::NST, NBLK = SM::NBLK;
-    constexpr uint32_t kSfCols = 8 + 8 * NBLK;              // TMEM columns of one stage's scales
-    constexpr uint32_t kTmemCols = 2 * BN + NST * kSfCols <= 256 ? 256 : 512;
-    static_assert(2 * BN + NST * kSfCols <= 512, "TMEM");
+    using SM = Smem<CG, BN>;
+    constexpr int NST = SM::NST, NBLK = SM::NBLK, BNC = BN / CG;
+    constexpr uint32_t kStageBytes = CG * ((BM + BNC) * 128 + (1 + NBLK) * 2 * kScaleBlock);
+    constexpr uint32_t kSfCols = 8 + 8 * NBLK;              // TMEM columns of one k-step's scales
+    constexpr uint32_t kTmemCols = 512;
+    constexpr uint32_t kSf0 = kTmemCols - NST * kSfCols;    // a set of scales per ring stage, at the end
+    constexpr uint32_t kAcc1 = 2 * BN <= kSf0 ? BN : kSf0 - BN;
+    constexpr bool kShared = kAcc1 < BN;                    // the accumulators share columns [kAcc1, BN)
+    static_assert(!kShared || BN - kAcc1 <= 128, "the shared columns are the first part each epilogue warp reads");
     SM& sm = *reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // through a shuffle the warp index is uniform to the compiler, which then keeps the MMA
+    // operands of its branch in uniform registers
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+    const int unit = blockIdx.x / CG, nunits = gridDim.x / CG;
     volatile int* abort_flag = &sm.abort_flag;
-    // rows, columns and steps past the operands read zeros (the tensor maps' fill); a k-step
-    // runs only the MMAs that k reaches
-    const int tiles_m = (int)((p.m + BM - 1) / BM), tiles_n = (p.n + BN - 1) / BN;
+    // rows, columns, steps and scales past the operands read zeros (the tensor maps' fill)
+    const int tiles_m = (int)((p.m + CG * BM - 1) / (CG * BM)), tiles_n = (p.n + BN - 1) / BN;
     const int ntiles = tiles_m * tiles_n;
     const int nk = (p.k + BK - 1) / BK;
-    const int groups = scale_col_groups(p.k);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NST; ++s) {
@@ -106,35 +136,42 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_u32(&sm.acc_full[b]), 1);
-            mbar_init(smem_u32(&sm.acc_empty[b]), EPI_WARPS);
+            mbar_init(smem_u32(&sm.acc_empty[b]), CG * EPI_WARPS);
         }
+        mbar_init(smem_u32(&sm.shared_empty), CG * EPI_WARPS);
         sm.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmA)) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW)) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmO)) : "memory");
+        for (const CUtensorMap* map : {&tmA, &tmW, &tmSA, &tmSW, &tmO})
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&sm.tmem_slot)), "r"(kTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(smem_u32(&sm.tmem_slot)), "r"(kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(smem_u32(&sm.tmem_slot)), "r"(kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        }
         tc_fence_before();
     }
     __syncthreads();
+    if (CG == 2) cluster_sync();     // the peer's barriers are initialised before anyone signals them
     tc_fence_after();
-    const uint32_t tmem = sm.tmem_slot;
+    // all 512 columns are this CTA's, so they start at 0: a constant, as MMA operands from shared
+    // memory would pass through vector registers
+    constexpr uint32_t tmem = 0;
 
     if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer
+        // ------------------------------------------------------------ TMA producer (every CTA)
         if (lane == 0) {
-            const int w_blocks = (p.n + 127) / 128;
             int it = 0;
             bool ok = true;
-            for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x) {
+            for (int t = unit; ok && t < ntiles; t += nunits) {
                 int tm, tn;
                 tile_coords(t, tiles_m, tiles_n, tm, tn);
-                const int wb = tn * BN / 128;               // first scale block of the tile's rows of w
-                const int nb = min(NBLK, w_blocks - wb);
+                const int rb = tm * CG + (int)rank;         // this CTA's rows of a, in blocks of 128
                 for (int kb = 0; kb < nk; ++kb, ++it) {
                     const int s = it % NST;
                     if (it >= NST &&
@@ -143,150 +180,173 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
                         break;
                     }
                     const uint32_t bar = smem_u32(&sm.full[s]);
-                    const uint32_t sf = (uint32_t)min(2, groups - 2 * kb) * kScaleBlock;
-                    mbar_expect_tx(bar, (BM + BN) * 128 + (1 + nb) * sf);
-                    tma_load_2d(smem_u32(sm.a[s]), &tmA, kb * 128, tm * BM, bar);
-                    tma_load_2d(smem_u32(sm.w[s]), &tmW, kb * 128, tn * BN, bar);
-                    bulk_load(smem_u32(sm.sa[s]), p.as + ((int64_t)tm * groups + 2 * kb) * kScaleBlock, sf, bar);
-                    for (int j = 0; j < nb; ++j)
-                        bulk_load(smem_u32(sm.sw[s][j]), p.ws + ((int64_t)(wb + j) * groups + 2 * kb) * kScaleBlock, sf,
-                                  bar);
+                    if (rank == 0) mbar_expect_tx(bar, kStageBytes);
+                    load_box<CG>(smem_u32(sm.sa[s]), &tmSA, kb * 256, rb, bar);
+                    load_box<CG>(smem_u32(sm.sw[s]), &tmSW, kb * 256, tn * BN / 128, bar);
+                    load_box<CG>(smem_u32(sm.a[s]), &tmA, kb * 128, rb * BM, bar);
+                    load_box<CG>(smem_u32(sm.w[s]), &tmW, kb * 128, tn * BN + (int)rank * BNC, bar);
                 }
             }
         }
     } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
+        // ------------------------------------------------------------ MMA issuer (even CTA)
         // the whole warp runs the loop, the elected lane issues, with descriptors as bases plus
         // stage and k offsets so they stay in uniform registers
-        const uint64_t ad0 = make_desc(smem_u32(sm.a[0]), 16, 1024, kSw128);
-        const uint64_t wd0 = make_desc(smem_u32(sm.w[0]), 16, 1024, kSw128);
-        const uint64_t sad0 = make_desc(smem_u32(sm.sa[0]), 16, 128, 0);
-        const uint64_t swd0 = make_desc(smem_u32(sm.sw[0]), 16, 128, 0);
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_mxlinear_error, kErr));
-        };
-        int it = 0, lt = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; ok && t < ntiles; t += gridDim.x, ++lt) {
-            const int buf = lt & 1;
-            int tm, tn;
-            tile_coords(t, tiles_m, tiles_n, tm, tn);
-            const uint32_t shift = (uint32_t)(tn * BN % 128) / 32;     // scale columns before the tile's first row
-            if (lt >= 2 && !wait(smem_u32(&sm.acc_empty[buf]), ((lt >> 1) - 1) & 1)) break;
-            tc_fence_after();
-            const uint32_t acc = tmem + buf * BN;
-            for (int kb = 0; kb < nk; ++kb, ++it) {
-                const int s = it % NST;
-                if (!wait(smem_u32(&sm.full[s]), (it / NST) & 1)) {
-                    ok = false;
-                    break;
-                }
+        if (rank == 0) {
+            const uint64_t ad0 = make_desc(smem_u32(sm.a[0]), 16, 1024, kSw128);
+            const uint64_t wd0 = make_desc(smem_u32(sm.w[0]), 16, 1024, kSw128);
+            const uint64_t sad0 = make_desc(smem_u32(sm.sa[0]), 16, 128, 0);
+            const uint64_t swd0 = make_desc(smem_u32(sm.sw[0]), 16, 128, 0);
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_mxlinear_error, kErr));
+            };
+            int it = 0, lt = 0;
+            bool ok = true, early = false;                  // early: the next step's data has been seen to be there
+            for (int t = unit; ok && t < ntiles; t += nunits, ++lt) {
+                const int buf = lt & 1;
+                int tm, tn;
+                tile_coords(t, tiles_m, tiles_n, tm, tn);
+                const uint32_t shift = (uint32_t)(tn * BN % 128) / 32;   // scale columns before the tile's first row
+                if (lt >= 2 && !wait(smem_u32(&sm.acc_empty[buf]), ((lt >> 1) - 1) & 1)) break;
+                if (kShared && lt >= 1 && !wait(smem_u32(&sm.shared_empty), (lt - 1) & 1)) break;
                 tc_fence_after();
-                const uint64_t ad = ad0 + (uint64_t)(s * (int)(sizeof(sm.a[0]) >> 4));
-                const uint64_t wd = wd0 + (uint64_t)(s * (int)(sizeof(sm.w[0]) >> 4));
-                const uint64_t sad = sad0 + (uint64_t)(s * (int)(sizeof(sm.sa[0]) >> 4));
-                const uint64_t swd = swd0 + (uint64_t)(s * (int)(sizeof(sm.sw[0]) >> 4));
-                const uint32_t sfa = tmem + 2 * BN + s * kSfCols, sfw = sfa + 8;
-                const int ng = min(2, groups - 2 * kb), nm = min(4, (p.k - kb * BK + 63) / 64);
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    if (g < ng) {
-                        tc_cp_scales_elect(sfa + 4 * g, sad + (uint64_t)(g * (kScaleBlock >> 4)));
-#pragma unroll
-                        for (int j = 0; j < NBLK; ++j)
-                            tc_cp_scales_elect(sfw + 4 * (g * NBLK + j),
-                                               swd + (uint64_t)((j * 2 + g) * (kScaleBlock >> 4)));
+                const uint32_t acc = tmem + buf * kAcc1;
+                for (int kb = 0; kb < nk; ++kb, ++it) {
+                    const int s = it % NST;
+                    if (!early && !wait(smem_u32(&sm.full[s]), (it / NST) & 1)) {
+                        ok = false;
+                        break;
                     }
+                    tc_fence_after();
+                    // ask for the next step before this one is issued: the answer takes ~200 clocks
+                    const int s1 = (it + 1) % NST;
+                    const bool next = mbar_test(smem_u32(&sm.full[s1]), ((it + 1) / NST) & 1);
+                    const uint32_t sfa = tmem + kSf0 + s * kSfCols, sfw = sfa + 8;
+                    // all four MMAs also in a partial last step, where they add zeros: with a branch
+                    // around each they took twice as long to issue
+                    tc_mxf4_step_elect<CG, NBLK>(
+                        acc, ad0 + (uint64_t)(s * (int)(sizeof(sm.a[0]) >> 4)),
+                        wd0 + (uint64_t)(s * (int)(sizeof(sm.w[0]) >> 4)),
+                        sad0 + (uint64_t)(s * (int)(sizeof(sm.sa[0]) >> 4)),
+                        swd0 + (uint64_t)(s * (int)(sizeof(sm.sw[0]) >> 4)), sfa, sfw, sfw + shift,
+                        make_idesc_mxf4(CG * BM, BN, 0), make_idesc_mxf4(CG * BM, BN, 2), (uint32_t)(kb > 0),
+                        smem_u32(&sm.empty[s]));
+                    early = __all_sync(0xffffffffu, next);
                 }
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    if (kk < nm)
-                        tc_mma_mxf4_elect(acc, ad + (uint64_t)(kk * 2), wd + (uint64_t)(kk * 2),
-                                          make_idesc_mxf4(BM, BN, (kk & 1) * 2), sfa + 4 * (kk >> 1),
-                                          sfw + 4 * NBLK * (kk >> 1) + shift, (kb > 0 || kk > 0) ? 1u : 0u);
-                tc_commit_elect(smem_u32(&sm.empty[s]));
+                if (ok) commit<CG>(smem_u32(&sm.acc_full[buf]));
             }
-            if (ok) tc_commit_elect(smem_u32(&sm.acc_full[buf]));
         }
     } else {
-        // ------------------------------------------------------------ epilogue
-        // Each warp turns 64 columns of its 32 rows at a time into bf16 in one of its two staging
-        // boxes (128-byte swizzle) and one lane stores the box; the map clips rows past m and
-        // columns past n.
-        const int ew = warp - 2, quarter = warp & 3;
+        // ------------------------------------------------------------ epilogue (every CTA)
+        // Two warps share each lane quarter (32 rows), one taking the even, one the odd 64-column
+        // parts of a tile.  A warp first reads its parts into registers, which frees the accumulator,
+        // then turns one after another into bf16 in its staging box (128-byte swizzle), which one
+        // lane stores; a second box a warp would cost a ring stage (95 against 86 us for
+        // 16384 x 7680 x 1536).  The map clips rows past m and columns past n.  The tile's bias is
+        // in shared memory before its accumulator is ready.
+        constexpr int PARTS = (BN / 64 + 1) / 2;            // parts of a warp, at most
+        const int ew = warp - 2, quarter = warp & 3, odd = ew >> 2;
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-        int lt = 0, nstore = 0;
-        for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++lt) {
+        float* bias = sm.bias[ew];
+        uint8_t* box = sm.x[ew];
+        int lt = 0;
+        for (int t = unit; t < ntiles; t += nunits, ++lt) {
             const int buf = lt & 1;
             int tm, tn;
             tile_coords(t, tiles_m, tiles_n, tm, tn);
+            const int64_t row0 = ((int64_t)tm * CG + rank) * BM + quarter * 32;
+            const int col0 = tn * BN;
+            __syncwarp();                                   // every lane has read the last tile's bias
+            for (int c = lane * 8; c < BN; c += 256) {      // n is a multiple of 8
+                float bv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (p.bias && col0 + c < p.n) load8_nc(p.bias + col0 + c, bv);
+                store8_f32(bias + c, bv);
+            }
+            __syncwarp();
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.acc_full[buf]), (lt >> 1) & 1, abort_flag,
                                                    &g_mxlinear_error, kErr)))
                 break;
             tc_fence_after();
-            const int64_t row0 = (int64_t)tm * BM + quarter * 32;
-            const int col0 = tn * BN;
-            if (row0 < p.m) {
-#pragma unroll 1
-                for (int c = 0; c < BN / 64; ++c) {
-                    if (col0 + c * 64 >= p.n) break;
-                    float v[64];
-                    tmem_ld32(tmem + buf * BN + c * 64 + lane_off, v);
-                    tmem_ld32(tmem + buf * BN + c * 64 + 32 + lane_off, v + 32);
+            // the first accumulator's last two parts and the second one's first two hold the columns
+            // both share: each warp reads its one of them first and says so
+            const bool reversed = kShared && buf == 0;
+            float v[PARTS][64];
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                const int c = 2 * (reversed ? PARTS - 1 - i : i) + odd;
+                if (c < BN / 64) {
+                    tmem_ld32(tmem + buf * kAcc1 + c * 64 + lane_off, v[i]);
+                    tmem_ld32(tmem + buf * kAcc1 + c * 64 + 32 + lane_off, v[i] + 32);
                     tmem_wait_ld();
-                    if (p.bias) {
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            const int cb = col0 + c * 64 + q * 8;   // n is a multiple of 8
-                            if (cb < p.n) {
-                                float bv[8];
-                                load8_nc(p.bias + cb, bv);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) v[q * 8 + j] += bv[j];
-                            }
-                        }
-                    }
-                    uint8_t* box = sm.x + (ew * 2 + (nstore & 1)) * 32 * 128;
-                    ++nstore;
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                }
+                if (i == PARTS - 1 || (kShared && i == 0)) {
+                    tc_fence_before();
                     __syncwarp();
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = pack8(v + q * 8);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tmO, smem_u32(box), col0 + c * 64, (int)row0);
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    }
+                    if (lane == 0) arrive_issuer<CG>(smem_u32(i == PARTS - 1 ? &sm.acc_empty[buf] : &sm.shared_empty), rank);
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sm.acc_empty[buf]));
+            if (row0 >= p.m) continue;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                const int c = 2 * (reversed ? PARTS - 1 - i : i) + odd;
+                if (c >= BN / 64 || col0 + c * 64 >= p.n) continue;
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    const float4 b = *reinterpret_cast<const float4*>(bias + c * 64 + q * 4);
+                    v[i][q * 4] += b.x;
+                    v[i][q * 4 + 1] += b.y;
+                    v[i][q * 4 + 2] += b.z;
+                    v[i][q * 4 + 3] += b.w;
+                }
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = pack8(v[i] + q * 8);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_2d(&tmO, smem_u32(box), col0 + c * 64, (int)row0);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+            }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync();     // no CTA leaves while its peer's MMAs or arrivals may still touch it
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+        if constexpr (CG == 1)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sm.tmem_slot), "r"(kTmemCols));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(sm.tmem_slot), "r"(kTmemCols));
     }
 }
 
-bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows, int cols, int64_t ld_bytes,
-              int box_rows, int box_cols) {
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, int64_t rows,
+              int64_t cols, int64_t ld_bytes, int box_rows, int box_cols) {
     auto fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld_bytes};
     cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     cuuint32_t es[2] = {1, 1};
-    return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// codes of a [rows, k] operand: 128-byte-wide boxes
+bool code_map(CUtensorMap* map, const void* codes, int64_t rows, int k, int box_rows) {
+    return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, codes, rows, k / 2, k / 2, box_rows, 128);
+}
+// its scales as rows of 512-byte blocks: two blocks (one k-step) of box_blocks block rows
+bool scale_map(CUtensorMap* map, const void* scales, int64_t rows, int k, int box_blocks) {
+    const int64_t words = (int64_t)scale_col_groups(k) * (kScaleBlock / 4);
+    return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, scales, scale_row_blocks(rows), words,
+                    words * 4, box_blocks, 2 * kScaleBlock / 4);
 }
 
 constexpr int kMaxDevices = 64;
@@ -300,35 +360,78 @@ int current_device(int* sms) {
     return dev;
 }
 
-template <int BN>
-int launch(const CUtensorMap& ma, const CUtensorMap& mo, const void* w, const Args& p, int dev, int sms,
-           cudaStream_t s) {
-    static std::atomic<bool> ready[kMaxDevices];            // the kernel's shared memory size is set, per device
-    constexpr int smem = (int)sizeof(Smem<BN>) + 1024;
-    if (!ready[dev].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(linear_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) {
-            record_cuda_error(e);
+struct Call {
+    const void *a, *as, *w, *ws;
+    CUtensorMap out;
+    Args p;
+    int dev, sms;
+    cudaStream_t stream;
+};
+
+template <int CG, int BN>
+int launch(const Call& c) {
+    // units (CTAs or pairs) resident at once, asked once per device; 0: not asked yet
+    static std::atomic<int> resident[kMaxDevices];
+    const Args& p = c.p;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = sizeof(Smem<CG, BN>) + 1024;
+    cfg.stream = c.stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int units = resident[c.dev].load(std::memory_order_acquire);
+    if (units == 0) {
+        cudaError_t e = cudaFuncSetAttribute(linear_kernel<CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)cfg.dynamicSmemBytes);
+        units = c.sms / CG;
+        if (e == cudaSuccess && CG == 2) {
+            cfg.gridDim = dim3(CG * units);
+            e = cudaOccupancyMaxActiveClusters(&units, linear_kernel<CG, BN>, &cfg);
+        }
+        if (e != cudaSuccess || units <= 0) {
+            record_cuda_error(e != cudaSuccess ? e : cudaErrorInvalidConfiguration);
             return VDIT_ERR_LAUNCH;
         }
-        ready[dev].store(true, std::memory_order_release);
+        resident[c.dev].store(units, std::memory_order_release);
     }
-    CUtensorMap mw;
-    if (!make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, p.n, p.k / 2, p.k / 2, BN, 128)) return VDIT_ERR_DRIVER;
-    const int64_t tiles = ((p.m + BM - 1) / BM) * ((p.n + BN - 1) / BN);
-    if (tiles > INT32_MAX - 1024) return VDIT_ERR_UNSUPPORTED;
-    linear_kernel<BN><<<(unsigned)std::min<int64_t>(tiles, sms), kThreads, smem, s>>>(ma, mw, mo, p);
+    CUtensorMap ma, mw, msa, msw;
+    if (!code_map(&ma, c.a, p.m, p.k, BM) || !code_map(&mw, c.w, p.n, p.k, BN / CG) ||
+        !scale_map(&msa, c.as, p.m, p.k, 1) || !scale_map(&msw, c.ws, p.n, p.k, Smem<CG, BN>::NBLK))
+        return VDIT_ERR_DRIVER;
+    const int64_t tiles = ((p.m + CG * BM - 1) / (CG * BM)) * ((p.n + BN - 1) / BN);
+    if (tiles > INT32_MAX / 2) return VDIT_ERR_UNSUPPORTED;
+    cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(tiles, units)));
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_kernel<CG, BN>, ma, mw, msa, msw, c.out, p);
+    if (e != cudaSuccess) {
+        record_cuda_error(e);
+        return VDIT_ERR_LAUNCH;
+    }
     count_launches(1);
     return check_launch();
 }
 
-// Tile width: 192 columns, or narrower ones when 192-column tiles would leave SMs idle and the
-// narrower fill more of them (few rows: the weight is then read by more SMs).
-int pick_bn(int64_t m, int n, int sms) {
-    const int64_t tiles_m = (m + BM - 1) / BM;
-    for (int bn : {192, 128})
-        if (tiles_m * ((n + bn - 1) / bn) >= sms) return bn;
-    return 64;
+// Tile for an [m, n] output: of the pairs' widths and the single CTA's 64 columns the one with
+// the least estimated time, rounds of tiles over the GPU x the time of a tile.
+int pick_tile(int64_t m, int n, int sms) {
+    const int widths[4] = {256, 192, 128, 64};
+    const double cost[4] = {1.0, 0.8, 0.6, 0.35};
+    int best = 64;
+    double best_t = 1e300;
+    for (int i = 0; i < 4; ++i) {
+        const int cg = widths[i] == 64 ? 1 : 2;
+        const int64_t tiles = ((m + cg * BM - 1) / (cg * BM)) * ((n + widths[i] - 1) / widths[i]);
+        const int64_t units = std::max(1, sms / cg);
+        const double t = (double)((tiles + units - 1) / units) * cost[i];
+        if (t < best_t) {
+            best_t = t;
+            best = widths[i];
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -362,16 +465,14 @@ extern "C" int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, cons
     int sms;
     const int dev = current_device(&sms);
     if (dev < 0) return VDIT_ERR_UNSUPPORTED;
-    CUtensorMap ma, mo;
-    if (!make_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a_codes, m, k / 2, k / 2, BM, 128) ||
-        !make_map(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, m, n, ldo * 2, 32, 64))
+    Call c{a_codes, a_scales, w_codes, w_scales, {}, {static_cast<const __nv_bfloat16*>(bias), m, n, k}, dev, sms,
+           static_cast<cudaStream_t>(stream)};
+    if (!make_map(&c.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, out, m, n, ldo * 2, 32, 64))
         return VDIT_ERR_DRIVER;
-    const Args p{static_cast<const uint8_t*>(a_scales), static_cast<const uint8_t*>(w_scales),
-                 static_cast<const __nv_bfloat16*>(bias), m, n, k};
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    switch (pick_bn(m, n, sms)) {
-        case 192: return launch<192>(ma, mo, w_codes, p, dev, sms, s);
-        case 128: return launch<128>(ma, mo, w_codes, p, dev, sms, s);
-        default: return launch<64>(ma, mo, w_codes, p, dev, sms, s);
+    switch (pick_tile(m, n, sms)) {
+        case 256: return launch<2, 256>(c);
+        case 192: return launch<2, 192>(c);
+        case 128: return launch<2, 128>(c);
+        default: return launch<1, 64>(c);
     }
 }

@@ -40,6 +40,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+// whether the phase has completed, without waiting (try_wait may suspend the thread for a while)
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // Bounded wait: polls at most kSpinLimit times.  Returns false when the CTA
 // aborted (another thread's wait ran out) or when this wait runs out; then it
 // raises the CTA abort flag and records `code` in the device error word `err`.
@@ -270,37 +283,6 @@ __host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int sf) {
            ((uint32_t)(m >> 7) << 27) | ((uint32_t)sf << 29);
 }
 
-// D (TMEM) += (A * its scales) (B * its scales), K = 64 (two blocks of 32 a row), issued by the
-// elected lane of a converged warp
-__device__ __forceinline__ void tc_mma_mxf4_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                                  uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accum) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accum)
-        : "memory");
-}
-
-// 32 rows x 16 bytes of shared memory -> 4 TMEM columns of lanes 0..31, repeated in the other
-// three lane quarters; ordered before the MMAs the same lane issues after it
-__device__ __forceinline__ void tc_cp_scales_elect(uint32_t tmem, uint64_t desc) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}"
-        ::"r"(tmem), "l"(desc)
-        : "memory");
-}
-
-// untiled bulk copy (16-byte aligned, a multiple of 16 bytes) counted on an mbarrier of this CTA
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-
 // ---------------------------------------------------------------- CTA pairs (cta_group::2)
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -372,6 +354,110 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t cta_mask) 
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"(cta_mask)
                  : "memory");
+}
+
+// One k-step of the block-scaled GEMM, issued by the elected lane of a converged warp: the scales of
+// 256 columns of A and B from shared memory to TMEM (tcgen05.cp 32x128b.warpx4: 32 rows x 16 bytes to
+// 4 columns of lanes 0..31, repeated in the other lane quarters), then
+//   D (TMEM) += (A * its scales) (B * its scales)
+// in four MMAs of K = 64, which find the scales of one 128-column group after the other, in the low
+// and the high halves of its words, and a commit to `bar`.  NBLK: 128-row scale blocks of B; its two
+// groups lie 512 bytes apart in shared memory, its blocks 1024.  sfb_rows: the TMEM word of B's
+// first row.  CG 2: issued in the even CTA of a pair, whose CTAs each hold 128 rows of A, half the
+// rows of B, the scales of their own rows of A and those of all rows of B; the commit reaches both.
+// All in one statement: with an elect.sync for each instruction a step took 330 clocks to issue.
+template <int CG, int NBLK>
+__device__ __forceinline__ void tc_mxf4_step_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint64_t sa_desc,
+                                                   uint64_t sb_desc, uint32_t sfa, uint32_t sfb, uint32_t sfb_rows,
+                                                   uint32_t idesc_lo, uint32_t idesc_hi, uint32_t accum, uint32_t bar) {
+    static_assert((CG == 1 && NBLK == 1) || (CG == 2 && (NBLK == 1 || NBLK == 2)), "");
+    if constexpr (CG == 1 && NBLK == 1)
+        asm volatile(
+            "{\n\t.reg .pred e, p, q;\n\t.reg .b32 t, u;\n\t.reg .b64 x, y;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "setp.ne.b32 p, %10, 0;\n\t"
+            "setp.eq.b32 q, 0, 0;\n\t"
+            "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%5], %3;\n\t"
+            "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%6], %4;\n\t"
+            "add.s32 t, %5, 4;\n\t"
+            "add.s64 x, %3, 32;\n\t"
+            "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [t], x;\n\t"
+            "add.s32 t, %6, 4;\n\t"
+            "add.s64 x, %4, 32;\n\t"
+            "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [t], x;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %8, [%5], [%7], p;\n\t"
+            "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %9, [%5], [%7], q;\n\t"
+            "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+            "add.s32 t, %5, 4;\n\tadd.s32 u, %7, 4;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %8, [t], [u], q;\n\t"
+            "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+            "add.s32 t, %5, 4;\n\tadd.s32 u, %7, 4;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %9, [t], [u], q;\n\t"
+            "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%11];\n\t}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "l"(sa_desc), "l"(sb_desc), "r"(sfa), "r"(sfb), "r"(sfb_rows), "r"(idesc_lo),
+              "r"(idesc_hi), "r"(accum), "r"(bar)
+            : "memory");
+    else if constexpr (CG == 2 && NBLK == 1)
+        asm volatile(
+            "{\n\t.reg .pred e, p, q;\n\t.reg .b32 t, u;\n\t.reg .b64 x, y;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "setp.ne.b32 p, %10, 0;\n\t"
+            "setp.eq.b32 q, 0, 0;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%5], %3;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%6], %4;\n\t"
+            "add.s32 t, %5, 4;\n\t"
+            "add.s64 x, %3, 32;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [t], x;\n\t"
+            "add.s32 t, %6, 4;\n\t"
+            "add.s64 x, %4, 32;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [t], x;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %8, [%5], [%7], p;\n\t"
+            "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %9, [%5], [%7], q;\n\t"
+            "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+            "add.s32 t, %5, 4;\n\tadd.s32 u, %7, 4;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %8, [t], [u], q;\n\t"
+            "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+            "add.s32 t, %5, 4;\n\tadd.s32 u, %7, 4;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %9, [t], [u], q;\n\t"
+            "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%11], %12;\n\t}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "l"(sa_desc), "l"(sb_desc), "r"(sfa), "r"(sfb), "r"(sfb_rows), "r"(idesc_lo),
+              "r"(idesc_hi), "r"(accum), "r"(bar), "h"((uint16_t)3)
+            : "memory");
+    else if constexpr (CG == 2 && NBLK == 2)
+        asm volatile(
+            "{\n\t.reg .pred e, p, q;\n\t.reg .b32 t, u;\n\t.reg .b64 x, y;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "setp.ne.b32 p, %10, 0;\n\t"
+            "setp.eq.b32 q, 0, 0;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%5], %3;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%6], %4;\n\t"
+            "add.s32 t, %6, 4;\n\t"
+            "add.s64 x, %4, 64;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [t], x;\n\t"
+            "add.s32 t, %5, 4;\n\t"
+            "add.s64 x, %3, 32;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [t], x;\n\t"
+            "add.s32 t, %6, 8;\n\t"
+            "add.s64 x, %4, 32;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [t], x;\n\t"
+            "add.s32 t, %6, 12;\n\t"
+            "add.s64 x, %4, 96;\n\t"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [t], x;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %8, [%5], [%7], p;\n\t"
+            "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %9, [%5], [%7], q;\n\t"
+            "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+            "add.s32 t, %5, 4;\n\tadd.s32 u, %7, 8;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %8, [t], [u], q;\n\t"
+            "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+            "add.s32 t, %5, 4;\n\tadd.s32 u, %7, 8;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %9, [t], [u], q;\n\t"
+            "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%11], %12;\n\t}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "l"(sa_desc), "l"(sb_desc), "r"(sfa), "r"(sfb), "r"(sfb_rows), "r"(idesc_lo),
+              "r"(idesc_hi), "r"(accum), "r"(bar), "h"((uint16_t)3)
+            : "memory");
 }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link)
