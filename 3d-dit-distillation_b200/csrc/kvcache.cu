@@ -7,6 +7,8 @@
 // consecutive: what one query head reads.
 #include <math.h>
 
+#include <atomic>
+
 #include "mx.cuh"
 #include "tc.cuh"
 
@@ -21,6 +23,7 @@ using namespace mx;
 
 constexpr int kErrIndex = 0x4B56;   // "KV": a slot, page or length outside the cache
 constexpr int kThreads = 256;
+constexpr int kMaxSplits = 1024;
 
 struct Cache {
     uint8_t *k, *v, *ks, *vs;
@@ -132,15 +135,29 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 
 // ------------------------------------------------------------------ single-query attention
 // One query per sequence and head over the cached keys of the sequence's pages: a stream of
-// head_dim * bits / 8 + head_dim / 32 bytes a key, twice, bound by HBM.  A CTA takes one
-// sequence, one key head, up to GT of the queries that share it and one range ("split") of the
-// sequence's keys.  A lane holds 16 channels (one load of 16 or 8 bytes; half a block, so one
-// scale), LPK lanes a key, and every group of LPK lanes runs its own online softmax in fp32 over
-// the keys it sees; the groups' states (max, sum, weighted values) are joined once at the end.
+// head_dim * bits / 8 + head_dim / 32 bytes a key, twice, bound by HBM once the arithmetic keeps up.
+// In fp32 on the CUDA cores it did not (an unpack, a conversion and an FMA an element and query: 312 us
+// for 16 sequences of up to 32768 keys, 12 x 128 heads, 8 bits; 53 us for 16 of up to 6082 with four
+// queries a key head), so both products run on mma.sync m16n8k16: a pair of elements is one
+// conversion to f16 (exact for both element types) and up to 8 queries of a key head share it.
+//
+// A CTA takes one sequence, one key head, up to 8 of its queries and one range ("split") of the keys.
+// Its warps are independent until the end: each takes every fourth group of 16 consecutive keys
+// (they lie in one page), copied by cp.async into the warp's own ring, rows padded to an odd number
+// of 16-byte chunks so that the fragment reads spread over the banks.  Per group and 32-channel block:
+//   S = K Q^T   16 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
+//               query by a power of two that puts its largest channel at 2^13: exact but for
+//               channels 2^27 below that one
+//   O += V^T P  channels x queries, P = 2^(s - m) in f16 (a weight is off by 2^-12 of itself, an
+//               eighth of the output's own rounding), each key's weight times its value scale
+//               relative to the group's largest, which multiplies the product in fp32
+// Channels and keys map to fragment indices so that a lane reads consecutive bytes.  m is raised
+// only by a score more than 1 above it (the weights stay below 2, the f16 ones, times 2^14, below
+// 2^15): exact, as every term uses the same m.
 constexpr int kWarps = 4;
-constexpr int kUnroll = 4;                   // keys in flight per lane: 2 x kUnroll loads
-
-template <int HD> constexpr int lanes_per_key() { return HD == 32 ? 2 : HD == 64 ? 4 : 8; }
+constexpr int kStages = 3;                   // groups of a warp in its ring
+constexpr int kQ = 8;                        // queries of a CTA
+constexpr int kGroup = 16;                   // keys of a group
 
 struct AttnArgs {
     const __nv_bfloat16* q;
@@ -167,254 +184,382 @@ __device__ __forceinline__ int64_t length_of(const AttnArgs& a, int page_size, i
     return n;
 }
 
-// 16 channels' codes -> 8 f16 pairs
-template <int BITS> struct Codes;
-template <> struct Codes<8> {
-    uint4 u;
-    __device__ __forceinline__ void load(const uint8_t* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
-    __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void decode(__half2* h) const {
-        decode4_e4m3(u.x, h);
-        decode4_e4m3(u.y, h + 2);
-        decode4_e4m3(u.z, h + 4);
-        decode4_e4m3(u.w, h + 6);
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// an 8 x 8 matrix of 16-bit elements, two of a row a lane, to its transpose
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 8 consecutive channels of a key to 4 f16 pairs
+template <int BITS>
+__device__ __forceinline__ void key_pairs(const uint8_t* p, uint32_t* h) {
+    if (BITS == 8) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        decode4_e4m3(u.x, reinterpret_cast<__half2*>(h));
+        decode4_e4m3(u.y, reinterpret_cast<__half2*>(h) + 2);
+    } else {
+        decode8_e2m1(*reinterpret_cast<const uint32_t*>(p), reinterpret_cast<__half2*>(h));
     }
-};
-template <> struct Codes<4> {
-    uint2 u;
-    __device__ __forceinline__ void load(const uint8_t* p) { u = __ldg(reinterpret_cast<const uint2*>(p)); }
-    __device__ __forceinline__ void zero() { u = make_uint2(0, 0); }
-    __device__ __forceinline__ void decode(__half2* h) const {
-        decode8_e2m1(u.x, h);
-        decode8_e2m1(u.y, h + 4);
+}
+
+// 4 consecutive channels of two keys' values to f16 pairs (first key, second key) of each channel
+template <int BITS>
+__device__ __forceinline__ void value_pairs(const uint8_t* p0, const uint8_t* p1, uint32_t* h) {
+    if (BITS == 8) {
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(p0), b = *reinterpret_cast<const uint32_t*>(p1);
+        decode4_e4m3(__byte_perm(a, b, 0x5140), reinterpret_cast<__half2*>(h));
+        decode4_e4m3(__byte_perm(a, b, 0x7362), reinterpret_cast<__half2*>(h) + 2);
+    } else {
+        const uint32_t a = *reinterpret_cast<const uint16_t*>(p0), b = *reinterpret_cast<const uint16_t*>(p1);
+        // bytes: channels 0, 2 of both keys, then 1, 3
+        const uint32_t even = (a & 0x0f0fu) | ((b << 4) & 0xf0f0u), od = ((a >> 4) & 0x0f0fu) | (b & 0xf0f0u);
+        __half2 t[4];
+        decode8_e2m1(even | (od << 16), t);
+        h[0] = *reinterpret_cast<uint32_t*>(&t[0]);
+        h[2] = *reinterpret_cast<uint32_t*>(&t[1]);
+        h[1] = *reinterpret_cast<uint32_t*>(&t[2]);
+        h[3] = *reinterpret_cast<uint32_t*>(&t[3]);
     }
+}
+
+// shared memory of a warp's ring and of the whole CTA
+template <int HD, int BITS>
+struct Ring {
+    static constexpr int W = HD * BITS / 8, CH = W / 16, NB = HD / kBlock;
+    static constexpr int PITCH = CH % 2 ? W : W + 16;
+    static constexpr int V = kGroup * PITCH, KS = 2 * V, VS = KS + kGroup * NB, STAGE = VS + kGroup * NB;
+    static constexpr int WARP = kStages * STAGE;
+    static constexpr int STATES = kWarps * kQ * (HD + 2) * 4;           // the warps' states, over the rings
+    static constexpr int BYTES = (kWarps * WARP > STATES ? kWarps * WARP : STATES);
 };
 
-template <int HD, int BITS, int GT>
+template <int HD, int BITS>
 __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a) {
-    constexpr int LPK = lanes_per_key<HD>(), KPW = 32 / LPK, KEYS = kWarps * KPW;
-    const int split = blockIdx.x, chunks = (a.group + GT - 1) / GT;
-    const int kh = blockIdx.y / chunks, g0 = (blockIdx.y % chunks) * GT, b = blockIdx.z;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, li = lane % LPK;
-    const bool active = li * 16 < HD;
-    const int ng = min(GT, a.group - g0);                   // live queries of this CTA
+    using R = Ring<HD, BITS>;
+    constexpr int NB = R::NB;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int live[kWarps][kStages];                   // keys of a group that count
+    const int split = blockIdx.x, chunks = (a.group + kQ - 1) / kQ;
+    const int kh = blockIdx.y / chunks, q0 = (blockIdx.y % chunks) * kQ, b = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int nq = min(kQ, a.group - q0);
     const int64_t len = length_of(a, c.page_size, b);
-    const int64_t per = ((len + a.splits - 1) / a.splits + KEYS - 1) / KEYS * KEYS;
+    constexpr int kStep = kWarps * kGroup;
+    const int64_t per = ((len + a.splits - 1) / a.splits + kStep - 1) / kStep * kStep;
     const int64_t k0 = min(len, split * per), k1 = min(len, k0 + per);
 
-    float2 q[GT][8];
+    // query g of this lane as the B fragments of S: per block four f16 pairs of channels t * 8 ...
+    uint32_t q[NB][4];
+    float c0, c1;                                           // score units of queries 2t and 2t + 1
+    {
+        float f[NB][8];
+        uint32_t top = 0;
 #pragma unroll
-    for (int g = 0; g < GT; ++g) {
-        float f[16];
+        for (int i = 0; i < NB; ++i) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) f[j] = 0.f;
-        if (active && g < ng) {
-            const __nv_bfloat16* p = a.q + b * a.ldq + (int64_t)(kh * a.group + g0 + g) * HD + li * 16;
-            load8(p, f);
-            load8(p + 8, f + 8);
+            for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
+            if (g < nq) load8(a.q + b * a.ldq + (int64_t)(kh * a.group + q0 + g) * HD + i * 32 + t * 8, f[i]);
+            top = max(top, amax8(f[i]));
         }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = top >> 23;
+        const uint32_t up = e == 0 || e == 255 ? 127u : min(253u, 267u - e);    // exponent field of the factor
+        const float unit = __uint_as_float((254u - up) << 23) * a.scale_log2;
+        c0 = __shfl_sync(0xffffffffu, unit, 8 * t);
+        c1 = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+        const float fac = __uint_as_float(up << 23);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[g][j] = make_float2(f[2 * j] * a.scale_log2, f[2 * j + 1] * a.scale_log2);
-    }
-    float m[GT], l[GT];
-    float2 o[GT][8];
+        for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int g = 0; g < GT; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[g][j] = make_float2(0.f, 0.f);
+            for (int j = 0; j < 4; ++j) q[i][j] = pack_f16(f[i][2 * j] * fac, f[i][2 * j + 1] * fac);
     }
 
+    uint8_t* ring = smem + warp * R::WARP;
+    const int n = (int)((k1 - k0 + kGroup - 1) / kGroup);   // groups of the split
+    const int mine = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;
     const int32_t* table = a.table + b * a.ldt;
-    // the loop bound is uniform across the warp (the shuffles below need every lane)
-    for (int64_t wbase = k0 + warp * KPW; wbase < k1; wbase += (int64_t)KEYS * kUnroll) {
-        Codes<BITS> kc[kUnroll], vc[kUnroll];
-        uint32_t ksb[kUnroll], vsb[kUnroll];
-        bool ok[kUnroll];
+    int pages = -1;                                         // lane i: page of this warp's group 32j + i
+    auto issue = [&](int i) {                               // copy group i of this warp, if there is one
+        if (i < mine) {
+            if ((i & 31) == 0) {
+                const int64_t key = k0 + (int64_t)(warp + kWarps * (i + lane)) * kGroup;
+                pages = key < k1 ? __ldg(table + (key >> c.page_shift)) : -1;
+            }
+            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+            const int64_t key = k0 + (int64_t)(warp + kWarps * i) * kGroup;
+            const bool there = page >= 0 && page < c.pages;
+            const int s = i % kStages;
+            if (lane == 0) {
+                live[warp][s] = there ? (int)min((int64_t)kGroup, k1 - key) : 0;
+                if (!there) atomicExch(&g_kvcache_error, kErrIndex);
+            }
+            if (there) {
+                const int64_t row = ((int64_t)page * c.heads + kh) * c.page_size + (key & (c.page_size - 1));
+                const uint32_t dst = tc::smem_u32(ring + s * R::STAGE);
+                const uint8_t *ks = c.k + row * R::W, *vs = c.v + row * R::W;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t key = wbase + lane / LPK + u * KEYS;
-            ok[u] = key < k1;
-            int page = -1;
-            if (ok[u]) {
-                page = __ldg(table + (key >> c.page_shift));
-                if (page < 0 || page >= c.pages) {          // no such page: its keys are left out
-                    atomicExch(&g_kvcache_error, kErrIndex);
-                    ok[u] = false;
+                for (int j = 0; j < (kGroup * R::CH + 31) / 32; ++j) {
+                    const int chunk = lane + 32 * j;
+                    if (kGroup * R::CH % 32 == 0 || chunk < kGroup * R::CH) {
+                        const uint32_t to = dst + chunk / R::CH * R::PITCH + chunk % R::CH * 16;
+                        cp_async16(to, ks + chunk * 16);
+                        cp_async16(to + R::V, vs + chunk * 16);
+                    }
                 }
-            }
-            kc[u].zero();
-            vc[u].zero();
-            ksb[u] = vsb[u] = 0;
-            if (ok[u] && active) {
-                const int off = (int)(key & (c.page_size - 1));
-                const int64_t d = data_at<BITS>(c, page, kh, off) + li * 16 * BITS / 8;
-                const int64_t s = scale_at(c, page, kh, off) + li / 2;
-                kc[u].load(c.k + d);
-                vc[u].load(c.v + d);
-                ksb[u] = __ldg(c.ks + s);
-                vsb[u] = __ldg(c.vs + s);
+                const int part = lane & 15;
+                if (part < NB)
+                    cp_async16(dst + (lane < 16 ? R::KS : R::VS) + part * 16,
+                               (lane < 16 ? c.ks : c.vs) + row * NB + part * 16);
             }
         }
-        float s[kUnroll][GT];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // of queries 2t and 2t + 1
+    float o[2 * NB][4];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            __half2 h[8];
-            kc[u].decode(h);
-            const float sc = scale_value(ksb[u]);
+    for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
-            for (int g = 0; g < GT; ++g) {
-                float2 acc = make_float2(0.f, 0.f);
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc = tc::ffma2v(q[g][j], __half22float2(h[j]), acc);
-                float t = (acc.x + acc.y) * sc;
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    for (int i = 0; i < mine; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        issue(i + kStages - 1);                             // into the stage the last step has read
+        uint8_t* st = ring + (i % kStages) * R::STAGE;
+        const int nl = live[warp][i % kStages];
+        if (nl == 0) continue;
+        if (nl < kGroup) {
+            // keys past the end: their values and scales, whatever they hold, must not reach the sums
+            for (int r = nl; r < kGroup; ++r) {
+                for (int j = lane; j < R::W / 4; j += 32) *reinterpret_cast<uint32_t*>(st + R::V + r * R::PITCH + j * 4) = 0;
+                if (lane < NB) st[R::VS + r * NB + lane] = 0;
+            }
+            __syncwarp();
+        }
+        // S = K Q^T: this lane has keys g and g + 8 of queries 2t and 2t + 1
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = LPK / 2; w > 0; w >>= 1) t += __shfl_xor_sync(0xffffffffu, t, w);
-                s[u][g] = ok[u] ? t : -INFINITY;
+        for (int k = 0; k < NB; ++k) {
+            uint32_t ka[4], kb[4];
+            const uint8_t* p = st + g * R::PITCH + (k * 32 + t * 8) * BITS / 8;
+            key_pairs<BITS>(p, ka);
+            key_pairs<BITS>(p + 8 * R::PITCH, kb);
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t f0[4] = {ka[0], kb[0], ka[1], kb[1]}, f1[4] = {ka[2], kb[2], ka[3], kb[3]};
+            mma_f16(d, f0, q[k][0], q[k][1]);
+            mma_f16(d, f1, q[k][2], q[k][3]);
+            const float sa = scale_value(st[R::KS + g * NB + k]), sb = scale_value(st[R::KS + (g + 8) * NB + k]);
+            s[0] = fmaf(d[0], sa, s[0]);
+            s[1] = fmaf(d[1], sa, s[1]);
+            s[2] = fmaf(d[2], sb, s[2]);
+            s[3] = fmaf(d[3], sb, s[3]);
+        }
+        s[0] = g < nl ? s[0] * c0 : -INFINITY;
+        s[1] = g < nl ? s[1] * c1 : -INFINITY;
+        s[2] = g + 8 < nl ? s[2] * c0 : -INFINITY;
+        s[3] = g + 8 < nl ? s[3] * c1 : -INFINITY;
+        const float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
+        if (__any_sync(0xffffffffu, t0 > m0 + 1.f || t1 > m1 + 1.f)) {
+            float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) {
+                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, w));
+                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, w));
+            }
+            const float f0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
+            m0 = n0;
+            m1 = n1;
+            l0 *= f0;
+            l1 *= f1;
+#pragma unroll
+            for (int j = 0; j < 2 * NB; ++j) {
+                o[j][0] *= f0;
+                o[j][1] *= f1;
+                o[j][2] *= f0;
+                o[j][3] *= f1;
             }
         }
-        float p[kUnroll][GT];
+        const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+        const float p[4] = {exp2f(s[0] - r0), exp2f(s[1] - r1), exp2f(s[2] - r0), exp2f(s[3] - r1)};
+        l0 += p[0] + p[2];
+        l1 += p[1] + p[3];
+        // O += V^T P
 #pragma unroll
-        for (int g = 0; g < GT; ++g) {
-            float mn = m[g];
+        for (int k = 0; k < NB; ++k) {
+            const uint32_t ea = st[R::VS + g * NB + k], eb = st[R::VS + (g + 8) * NB + k];
+            uint32_t top = max(ea, eb);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) mn = fmaxf(mn, s[u][g]);
-            const float ref = mn == -INFINITY ? 0.f : mn;   // nothing seen yet: every weight is 0
-            const float f = exp2f(m[g] - ref);
-            l[g] *= f;
+            for (int w = 4; w < 32; w <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, w));
+            // 2^14 * 2^(e - top), 0 below the smallest normal number
+            const float fa = __uint_as_float((uint32_t)max(141 + (int)ea - (int)top, 0) << 23);
+            const float fb = __uint_as_float((uint32_t)max(141 + (int)eb - (int)top, 0) << 23);
+            const uint32_t b0 = transpose8(pack_f16(p[0] * fa, p[1] * fa));
+            const uint32_t b1 = transpose8(pack_f16(p[2] * fb, p[3] * fb));
+            uint32_t va[4], vb[4];                          // keys 2t, 2t + 1 and 2t + 8, 2t + 9
+            const uint8_t* v = st + R::V + 2 * t * R::PITCH + (k * 32 + g * 4) * BITS / 8;
+            value_pairs<BITS>(v, v + R::PITCH, va);
+            value_pairs<BITS>(v + 8 * R::PITCH, v + 9 * R::PITCH, vb);
+            const float unit = scale_value(top) * 6.103515625e-05f;             // 2^-14
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[g][j] = make_float2(o[g][j].x * f, o[g][j].y * f);
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t f[4] = {va[2 * h], va[2 * h + 1], vb[2 * h], vb[2 * h + 1]};
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_f16(d, f, b0, b1);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                p[u][g] = exp2f(s[u][g] - ref);
-                l[g] += p[u][g];
-            }
-            m[g] = mn;
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            __half2 h[8];
-            vc[u].decode(h);
-            const float sc = scale_value(vsb[u]);
-#pragma unroll
-            for (int g = 0; g < GT; ++g) {
-                const float w = p[u][g] * sc;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[g][j] = tc::ffma2v(__half22float2(h[j]), make_float2(w, w), o[g][j]);
+                for (int j = 0; j < 4; ++j) o[2 * k + h][j] = fmaf(d[j], unit, o[2 * k + h][j]);
             }
         }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 
-    // join the KPW groups of a warp in registers, then the warps through shared memory
-    __shared__ float sm[kWarps][GT], sl[kWarps][GT], so[kWarps][GT][HD];
+    // join the warps through shared memory
 #pragma unroll
-    for (int g = 0; g < GT; ++g) {
-        float mm = m[g];
+    for (int w = 4; w < 32; w <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, w);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, w);
+    }
+    __syncthreads();                                        // the rings are done with
+    float* ml = reinterpret_cast<float*>(smem);             // [warp][query][2]
+    float* so = ml + kWarps * kQ * 2;                       // [warp][query][HD]
+    if (g == 0) {
+        float* x = ml + (warp * kQ + 2 * t) * 2;
+        x[0] = m0;
+        x[1] = l0;
+        x[2] = m1;
+        x[3] = l1;
+    }
 #pragma unroll
-        for (int w = LPK; w < 32; w <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
-        const float f = m[g] == -INFINITY ? 0.f : exp2f(m[g] - mm);
-        float ll = l[g] * f;
-#pragma unroll
-        for (int w = LPK; w < 32; w <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float2 t = make_float2(o[g][j].x * f, o[g][j].y * f);
-#pragma unroll
-            for (int w = LPK; w < 32; w <<= 1) {
-                t.x += __shfl_xor_sync(0xffffffffu, t.x, w);
-                t.y += __shfl_xor_sync(0xffffffffu, t.y, w);
-            }
-            if (lane < LPK && active) {
-                so[warp][g][li * 16 + 2 * j] = t.x;
-                so[warp][g][li * 16 + 2 * j + 1] = t.y;
-            }
-        }
-        if (lane == 0) {
-            sm[warp][g] = mm;
-            sl[warp][g] = ll;
-        }
+    for (int j = 0; j < 2 * NB; ++j) {
+        float* x = so + (warp * kQ + 2 * t) * HD + j / 2 * 32 + g * 4 + (j & 1) * 2;
+        *reinterpret_cast<float2*>(x) = make_float2(o[j][0], o[j][2]);
+        *reinterpret_cast<float2*>(x + HD) = make_float2(o[j][1], o[j][3]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < ng * HD; i += kWarps * 32) {
-        const int g = i / HD, e = i - g * HD;
+    for (int i = threadIdx.x; i < nq * HD; i += kWarps * 32) {
+        const int j = i / HD, e = i - j * HD;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm[w][g]);
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml[(w * kQ + j) * 2]);
         float acc = 0.f, ll = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = sm[w][g] == -INFINITY ? 0.f : exp2f(sm[w][g] - mm);
-            acc += so[w][g][e] * f;
-            ll += sl[w][g] * f;
+            const float mw = ml[(w * kQ + j) * 2];
+            const float f = mw == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : exp2f(mw - mm);
+            acc += so[(w * kQ + j) * HD + e] * f;
+            ll += ml[(w * kQ + j) * 2 + 1] * f;
         }
-        const int h = kh * a.group + g0 + g;
+        const int h = kh * a.group + q0 + j;
         if (a.splits == 1) {
-            a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(len == 0 ? 0.f : acc / ll);
+            a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(ll == 0.f ? 0.f : acc / ll);
         } else {
-            float* p = a.ws + (((int64_t)b * a.heads + h) * a.splits + split) * (2 + HD);
-            p[2 + e] = acc;
+            float* x = a.ws + (((int64_t)b * a.heads + h) * a.splits + split) * (2 + HD);
+            x[2 + e] = acc;
             if (e == 0) {
-                p[0] = mm;
-                p[1] = ll;
+                x[0] = mm;
+                x[1] = ll;
             }
         }
     }
 }
 
-// joins the splits of one (sequence, head); a sequence without keys gives zeros
+// joins the splits of one (sequence, head); no keys give zeros
 template <int HD>
-__global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a, int page_size) {
-    const int h = blockIdx.x, b = blockIdx.y, e = threadIdx.x;
+__global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
+    __shared__ float weight[kMaxSplits];
+    __shared__ float red[2][HD / 32];
+    const int h = blockIdx.x, b = blockIdx.y, e = threadIdx.x, warp = e >> 5, lane = e & 31;
     const float* base = a.ws + ((int64_t)b * a.heads + h) * a.splits * (2 + HD);
     float mm = -INFINITY;
-    for (int i = 0; i < a.splits; ++i) mm = fmaxf(mm, base[i * (2 + HD)]);
-    float acc = 0.f, ll = 0.f;
-    for (int i = 0; i < a.splits; ++i) {
-        const float* p = base + i * (2 + HD);
-        const float f = p[0] == -INFINITY ? 0.f : exp2f(p[0] - mm);
-        ll += p[1] * f;
-        acc += p[2 + e] * f;
+    for (int i = e; i < a.splits; i += HD) mm = fmaxf(mm, base[i * (2 + HD)]);
+    mm = warp_max(mm);
+    if (lane == 0) red[0][warp] = mm;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < HD / 32; ++w) mm = fmaxf(mm, red[0][w]);
+    float ll = 0.f;
+    for (int i = e; i < a.splits; i += HD) {
+        const float mi = base[i * (2 + HD)];
+        const float f = mi == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : exp2f(mi - mm);
+        weight[i] = f;
+        ll += base[i * (2 + HD) + 1] * f;
     }
-    const int64_t len = length_of(a, page_size, b);
-    a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(len == 0 ? 0.f : acc / ll);
+    ll = warp_sum(ll);
+    if (lane == 0) red[1][warp] = ll;
+    __syncthreads();
+    ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < HD / 32; ++w) ll += red[1][w];
+    float acc = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < a.splits; ++i) acc = fmaf(base[i * (2 + HD) + 2 + e], weight[i], acc);
+    a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(ll == 0.f ? 0.f : acc / ll);
 }
 
-// queries of a CTA: the group, up to 4 (more would not fit the registers: 32 a query)
-int queries_per_cta(int group) { return group >= 3 ? 4 : group; }
-
-// Splits of a sequence's keys: enough CTAs for the whole GPU (8 of 4 warps on each of 148 SMs),
-// none with fewer than 128 keys of the longest sequence.
+// Splits of a sequence's keys: two rounds of the CTAs that fit the GPU (3 of 4 warps on each of 148
+// SMs), none with fewer than 128 keys of the longest sequence.
 int choose_splits(int batch, int heads, int kv_heads, int64_t longest) {
-    const int group = heads / kv_heads, gt = queries_per_cta(group);
-    const int64_t ctas = (int64_t)batch * kv_heads * ((group + gt - 1) / gt);
-    const int64_t want = (8 * 148 + ctas - 1) / ctas, by_len = (longest + 127) / 128;
+    const int group = heads / kv_heads;
+    const int64_t ctas = (int64_t)batch * kv_heads * ((group + kQ - 1) / kQ);
+    const int64_t want = (6 * 148 + ctas - 1) / ctas, by_len = (longest + 127) / 128;
     const int64_t s = want < by_len ? want : by_len;
-    return (int)(s < 1 ? 1 : s > 1024 ? 1024 : s);
+    return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
 }
+
+constexpr int kMaxDevices = 64;
 
 template <int HD, int BITS>
-void launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) {
-    const int gt = queries_per_cta(a.group);
-    const dim3 grid(a.splits, c.heads * ((a.group + gt - 1) / gt), batch);
-    if (gt == 1) attend_kernel<HD, BITS, 1><<<grid, kWarps * 32, 0, s>>>(c, a);
-    else if (gt == 2) attend_kernel<HD, BITS, 2><<<grid, kWarps * 32, 0, s>>>(c, a);
-    else attend_kernel<HD, BITS, 4><<<grid, kWarps * 32, 0, s>>>(c, a);
+int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) {
+    static std::atomic<bool> ready[kMaxDevices];            // the kernel's shared memory size is set, per device
+    constexpr int bytes = Ring<HD, BITS>::BYTES;
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) return VDIT_ERR_UNSUPPORTED;
+    if (e == cudaSuccess && bytes > 48 * 1024 && !ready[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(attend_kernel<HD, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) ready[dev].store(true, std::memory_order_release);
+    }
+    if (e != cudaSuccess) {
+        record_cuda_error(e);
+        return VDIT_ERR_LAUNCH;
+    }
+    const dim3 grid(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
+    attend_kernel<HD, BITS><<<grid, kWarps * 32, bytes, s>>>(c, a);
     count_launches(1);
     if (a.splits > 1) {
-        combine_kernel<HD><<<dim3(a.heads, batch), HD, 0, s>>>(a, c.page_size);
+        combine_kernel<HD><<<dim3(a.heads, batch), HD, 0, s>>>(a);
         count_launches(1);
     }
+    return check_launch();
 }
 
 // the cache's own checks; fills c
 int check_cache(void* k, void* v, void* ks, void* vs, int64_t pages, int32_t page_size, int32_t heads, int32_t hd,
                 int32_t bits, Cache* c) {
     if (!k || !v || !ks || !vs || pages < 1 || page_size < 1 || heads < 1 || hd < 1) return VDIT_ERR_ARG;
-    if ((bits != 4 && bits != 8) || hd % 32 || hd > 128 || (page_size & (page_size - 1)) || page_size > 1024 ||
+    if ((bits != 4 && bits != 8) || hd % 32 || hd > 128 || (page_size & (page_size - 1)) || page_size < 16 || page_size > 1024 ||
         heads > 4096 || pages > INT32_MAX)
         return VDIT_ERR_UNSUPPORTED;
-    if (!aligned16(k) || !aligned16(v)) return VDIT_ERR_ALIGN;
+    if (!aligned16(k) || !aligned16(v) || !aligned16(ks) || !aligned16(vs)) return VDIT_ERR_ALIGN;
     int shift = 0;
     while ((1 << shift) < page_size) ++shift;
     *c = Cache{static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), static_cast<uint8_t*>(ks), static_cast<uint8_t*>(vs),
@@ -527,12 +672,10 @@ extern "C" int vdit_attention_1q_cached(const void* q, int64_t ldq, const void* 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     auto run = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        if (bits == 4) launch_attend<HD, 4>(c, a, batch, s);
-        else launch_attend<HD, 8>(c, a, batch, s);
+        return bits == 4 ? launch_attend<HD, 4>(c, a, batch, s) : launch_attend<HD, 8>(c, a, batch, s);
     };
-    if (head_dim == 32) run(std::integral_constant<int, 32>{});
-    else if (head_dim == 64) run(std::integral_constant<int, 64>{});
-    else if (head_dim == 96) run(std::integral_constant<int, 96>{});
-    else run(std::integral_constant<int, 128>{});
-    return check_launch();
+    if (head_dim == 32) return run(std::integral_constant<int, 32>{});
+    if (head_dim == 64) return run(std::integral_constant<int, 64>{});
+    if (head_dim == 96) return run(std::integral_constant<int, 96>{});
+    return run(std::integral_constant<int, 128>{});
 }

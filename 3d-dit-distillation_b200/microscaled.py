@@ -179,7 +179,7 @@ def linear_mxfp4(a: Union[torch.Tensor, Mxfp4Tensor], w: Mxfp4Tensor, bias: Opti
 class MxKvCache:
     """A paged cache of keys and values held in 8 (e4m3) or 4 (e2m1) bits with a scale per 32
     channels.  Slot ``page * page_size + offset`` holds one row of ``kv_heads * head_dim``
-    channels.  ``page_size`` is a power of two up to 1024, ``head_dim`` 32, 64, 96 or 128.  Its
+    channels.  ``page_size`` is a power of two from 16 to 1024, ``head_dim`` 32, 64, 96 or 128.  Its
     buffers ``k``, ``v``, ``k_scales`` and ``v_scales`` stay where they are."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 8, device="cuda"):
@@ -187,8 +187,8 @@ class MxKvCache:
             raise ValueError(f"MxKvCache: bits must be 4 or 8, got {bits}")
         if head_dim not in (32, 64, 96, 128):
             raise ValueError(f"MxKvCache: head_dim must be 32, 64, 96 or 128, got {head_dim}")
-        if page_size < 1 or page_size > 1024 or page_size & (page_size - 1):
-            raise ValueError(f"MxKvCache: page_size must be a power of two up to 1024, got {page_size}")
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError(f"MxKvCache: page_size must be a power of two from 16 to 1024, got {page_size}")
         if pages < 1 or kv_heads < 1:
             raise ValueError(f"MxKvCache: needs pages and heads, got {pages} and {kv_heads}")
         self.pages, self.page_size, self.kv_heads, self.head_dim, self.bits = pages, page_size, kv_heads, head_dim, bits
@@ -266,8 +266,8 @@ def attention_1q_cached(q: torch.Tensor, cache: MxKvCache, page_table: torch.Ten
     sequence and head, ``q`` bf16 [B, heads * head_dim] (heads a multiple of the cache's; query head
     h reads key head h // (heads / kv_heads)), ``page_table`` int32 [B, P] (row stride free; 0, as of
     an expanded row, shares it), ``lengths`` int32 [B].  Key i of sequence b is in page
-    ``page_table[b, i // page_size]``; entries past a length are not read, and a sequence of length
-    0 gives zeros.  Pages outside the cache are left out and lengths outside the table are clipped
+    ``page_table[b, i // page_size]``; entries past a length are not read, and a sequence without
+    keys gives zeros.  Pages outside the cache are left out and lengths outside the table are clipped
     to it, both recorded in the device error word.  Returns bf16 [B, heads * head_dim]."""
     what = "attention_1q_cached"
     ldq = _rows_view(what, "q", q, (BF16,))

@@ -350,8 +350,8 @@ int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, const void* w_c
 /* A paged cache of keys and values in a microscaled format, bits 8 (e4m3) or 4 (e2m1).  Slot
  * page * page_size + offset holds one row of heads * head_dim channels: kc and vc are
  * [pages, heads, page_size, head_dim * bits / 8] bytes, k_scales and v_scales
- * [pages, heads, page_size, head_dim / 32] bytes.  page_size is a power of two up to 1024;
- * head_dim 32, 64, 96 or 128; kc, vc 16-byte aligned.
+ * [pages, heads, page_size, head_dim / 32] bytes.  page_size is a power of two from 16 to
+ * 1024; head_dim 32, 64, 96 or 128; all four buffers 16-byte aligned.
  *
  * write: rows k, v bf16 [n, ldk], [n, ldv] are quantised into slots[n]; a negative slot is
  * skipped, and no slot may appear twice among the others.  read: the rows the slots stand for, bf16

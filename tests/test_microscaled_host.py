@@ -50,7 +50,7 @@ def test_wrappers_refuse_what_they_cannot_take():
 
 
 def test_cache_refusals():
-    for kw in (dict(bits=6), dict(head_dim=80), dict(page_size=24), dict(page_size=2048), dict(pages=0),
+    for kw in (dict(bits=6), dict(head_dim=80), dict(page_size=24), dict(page_size=8), dict(page_size=2048), dict(pages=0),
                dict(kv_heads=0)):
         a = dict(pages=2, page_size=16, kv_heads=2, head_dim=64, bits=8, device="cpu")
         a.update(kw)
@@ -109,7 +109,7 @@ def test_c_entry_points_check_before_any_launch():
     assert lib.vdit_attention_1q_cached(*a) == -5
 
 
-@pytest.mark.parametrize("pages,page,heads,hd,bits", [(3, 16, 5, 96, 4), (7, 1, 2, 32, 8), (2, 1024, 3, 128, 8),
+@pytest.mark.parametrize("pages,page,heads,hd,bits", [(3, 16, 5, 96, 4), (7, 16, 2, 32, 8), (2, 1024, 3, 128, 8),
                                                        (70000, 128, 12, 128, 8)])
 def test_cache_addresses_stay_inside_and_apart(pages, page, heads, hd, bits):
     """The kernels' address arithmetic, ((page * heads + head) * page_size + offset) * width + element
