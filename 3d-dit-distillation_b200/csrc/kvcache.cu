@@ -7,6 +7,7 @@
 // consecutive: what one query head reads.
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "mx.cuh"
@@ -142,10 +143,11 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 // conversion to f16 (exact for both element types) and up to 8 queries of a key head share it.
 //
 // A CTA takes one sequence, one key head, up to 8 of its queries and one range ("split") of the keys.
-// Its warps are independent until the end: each takes every fourth group of 16 consecutive keys
-// (they lie in one page), copied by cp.async into the warp's own ring, rows padded to an odd number
-// of 16-byte chunks so that the fragment reads spread over the banks.  Per group and 32-channel block:
-//   S = K Q^T   16 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
+// Its warps are independent until the end: each takes every fourth group of 32 consecutive keys (two
+// halves of 16, each in one page), copied by cp.async into the warp's own ring, rows padded to an odd
+// number of 16-byte chunks so that the fragment reads spread over the banks.  Per group and
+// 32-channel block:
+//   S = K Q^T   32 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
 //               query by a power of two that puts its largest channel at 2^13: exact but for
 //               channels 2^27 below that one
 //   O += V^T P  channels x queries, P = 2^(s - m) in f16 (a weight is off by 2^-12 of itself, an
@@ -155,9 +157,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 // only by a score more than 1 above it (the weights stay below 2, the f16 ones, times 2^14, below
 // 2^15): exact, as every term uses the same m.
 constexpr int kWarps = 4;
-constexpr int kStages = 3;                   // groups of a warp in its ring
 constexpr int kQ = 8;                        // queries of a CTA
-constexpr int kGroup = 16;                   // keys of a group
+constexpr int kGroup = 32;                   // keys of a group
 
 struct AttnArgs {
     const __nv_bfloat16* q;
@@ -169,7 +170,7 @@ struct AttnArgs {
     const int32_t* lengths;                  // [batch]
     int max_pages;                           // entries of a table row
     int heads, group;                        // query heads, and how many share a key head
-    int splits;
+    int splits, per;                         // key ranges, and keys of each
     float scale_log2;
     float* ws;                               // [batch, heads, splits, 2 + hd] when splits > 1
 };
@@ -238,31 +239,50 @@ __device__ __forceinline__ void value_pairs(const uint8_t* p0, const uint8_t* p1
     }
 }
 
+// the NB scale bytes of a row in one word (NB = 3: two words' neighbours, the second one read for
+// nothing in some rows)
+template <int NB>
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* s, int row) {
+    if (NB == 4) return *reinterpret_cast<const uint32_t*>(s + row * 4);
+    if (NB == 2) return *reinterpret_cast<const uint16_t*>(s + row * 2);
+    if (NB == 1) return s[row];
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(s) + (row * 3 >> 2);
+    return __funnelshift_r(w[0], w[1], (row * 3 & 3) * 8);
+}
+// byte k of a word as 2^(byte - 127); 255 gives an infinity, which makes a NaN of the zeros that a
+// block with that scale holds
+__device__ __forceinline__ float word_scale(uint32_t w, int k) {
+    return __uint_as_float(max((k < 3 ? w >> (8 * k) & 255u : w >> 24) << 23, 0x00400000u));
+}
+
 // shared memory of a warp's ring and of the whole CTA
 template <int HD, int BITS>
 struct Ring {
     static constexpr int W = HD * BITS / 8, CH = W / 16, NB = HD / kBlock;
     static constexpr int PITCH = CH % 2 ? W : W + 16;
     static constexpr int V = kGroup * PITCH, KS = 2 * V, VS = KS + kGroup * NB, STAGE = VS + kGroup * NB;
-    static constexpr int WARP = kStages * STAGE;
+    // groups in the ring: what leaves room for three CTAs an SM, up to 4
+    static constexpr int STAGES = 19000 / STAGE > 4 ? 4 : 19000 / STAGE;
+    static_assert(STAGES >= 2, "");
+    static constexpr int WARP = STAGES * STAGE;
     static constexpr int STATES = kWarps * kQ * (HD + 2) * 4;           // the warps' states, over the rings
-    static constexpr int BYTES = (kWarps * WARP > STATES ? kWarps * WARP : STATES);
+    static constexpr int BYTES = (kWarps * WARP > STATES ? kWarps * WARP : STATES) + 16;   // scale_word reads past
 };
 
 template <int HD, int BITS>
 __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a) {
     using R = Ring<HD, BITS>;
-    constexpr int NB = R::NB;
+    constexpr int NB = R::NB, kStages = R::STAGES;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int live[kWarps][kStages];                   // keys of a group that count
+    __shared__ int live[kWarps][kStages][2];                // keys that count of the halves of a group
     const int split = blockIdx.x, chunks = (a.group + kQ - 1) / kQ;
     const int kh = blockIdx.y / chunks, q0 = (blockIdx.y % chunks) * kQ, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nq = min(kQ, a.group - q0);
-    const int64_t len = length_of(a, c.page_size, b);
+    asm volatile("griddepcontrol.launch_dependents;");
     constexpr int kStep = kWarps * kGroup;
-    const int64_t per = ((len + a.splits - 1) / a.splits + kStep - 1) / kStep * kStep;
-    const int64_t k0 = min(len, split * per), k1 = min(len, k0 + per);
+    const int len = (int)length_of(a, c.page_size, b);      // as int32 as the caller's
+    const int k0 = (int)min((int64_t)len, (int64_t)split * a.per), k1 = (int)min((int64_t)len, (int64_t)k0 + a.per);
 
     // query g of this lane as the B fragments of S: per block four f16 pairs of channels t * 8 ...
     uint32_t q[NB][4];
@@ -292,32 +312,33 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     }
 
     uint8_t* ring = smem + warp * R::WARP;
-    const int n = (int)((k1 - k0 + kGroup - 1) / kGroup);   // groups of the split
-    const int mine = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;
+    const int first = k0 + warp * kGroup;                   // this warp's groups start at first + i * kStep
+    const int mine = first < k1 ? (k1 - first + kStep - 1) / kStep : 0;
     const int32_t* table = a.table + b * a.ldt;
-    int pages = -1;                                         // lane i: page of this warp's group 32j + i
-    auto issue = [&](int i) {                               // copy group i of this warp, if there is one
+    int pages = -1;                                         // lane j: page of half j of 16 groups
+    auto issue = [&](int i, int s) {                        // copy group i of this warp, if there is one, to stage s
         if (i < mine) {
-            if ((i & 31) == 0) {
-                const int64_t key = k0 + (int64_t)(warp + kWarps * (i + lane)) * kGroup;
-                pages = key < k1 ? __ldg(table + (key >> c.page_shift)) : -1;
+            if ((i & 15) == 0) {
+                const int j = first + (i + (lane >> 1)) * kStep + (lane & 1) * 16;
+                pages = j < k1 ? __ldg(table + (j >> c.page_shift)) : -1;
             }
-            const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-            const int64_t key = k0 + (int64_t)(warp + kWarps * i) * kGroup;
-            const bool there = page >= 0 && page < c.pages;
-            const int s = i % kStages;
-            if (lane == 0) {
-                live[warp][s] = there ? (int)min((int64_t)kGroup, k1 - key) : 0;
-                if (!there) atomicExch(&g_kvcache_error, kErrIndex);
-            }
-            if (there) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int page = __shfl_sync(0xffffffffu, pages, (i & 15) * 2 + h);
+                const int key = first + i * kStep + h * 16;
+                const bool there = key < k1 && page >= 0 && page < c.pages;
+                if (lane == 0) {
+                    live[warp][s][h] = there ? min(16, k1 - key) : 0;
+                    if (key < k1 && !there) atomicExch(&g_kvcache_error, kErrIndex);
+                }
+                if (!there) continue;
                 const int64_t row = ((int64_t)page * c.heads + kh) * c.page_size + (key & (c.page_size - 1));
-                const uint32_t dst = tc::smem_u32(ring + s * R::STAGE);
+                const uint32_t dst = tc::smem_u32(ring + s * R::STAGE) + h * 16 * R::PITCH;
                 const uint8_t *ks = c.k + row * R::W, *vs = c.v + row * R::W;
 #pragma unroll
-                for (int j = 0; j < (kGroup * R::CH + 31) / 32; ++j) {
+                for (int j = 0; j < (16 * R::CH + 31) / 32; ++j) {
                     const int chunk = lane + 32 * j;
-                    if (kGroup * R::CH % 32 == 0 || chunk < kGroup * R::CH) {
+                    if (16 * R::CH % 32 == 0 || chunk < 16 * R::CH) {
                         const uint32_t to = dst + chunk / R::CH * R::PITCH + chunk % R::CH * 16;
                         cp_async16(to, ks + chunk * 16);
                         cp_async16(to + R::V, vs + chunk * 16);
@@ -325,7 +346,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
                 }
                 const int part = lane & 15;
                 if (part < NB)
-                    cp_async16(dst + (lane < 16 ? R::KS : R::VS) + part * 16,
+                    cp_async16(tc::smem_u32(ring + s * R::STAGE) + (lane < 16 ? R::KS : R::VS) + (h * NB + part) * 16,
                                (lane < 16 ? c.ks : c.vs) + row * NB + part * 16);
             }
         }
@@ -340,45 +361,62 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    for (int i = 0; i < kStages - 1; ++i) issue(i, i);
+    int cur = 0, next = kStages - 1;                        // the stage of this step and the one its copies go to
     for (int i = 0; i < mine; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();
-        issue(i + kStages - 1);                             // into the stage the last step has read
-        uint8_t* st = ring + (i % kStages) * R::STAGE;
-        const int nl = live[warp][i % kStages];
-        if (nl == 0) continue;
-        if (nl < kGroup) {
-            // keys past the end: their values and scales, whatever they hold, must not reach the sums
-            for (int r = nl; r < kGroup; ++r) {
+        issue(i + kStages - 1, next);                       // the stage the last step has read
+        uint8_t* st = ring + cur * R::STAGE;
+        const int nl[2] = {live[warp][cur][0], live[warp][cur][1]};
+        next = cur;
+        cur = cur == kStages - 1 ? 0 : cur + 1;
+        const bool whole = nl[0] + nl[1] == kGroup;
+        if (!whole) {
+            // keys that do not count: their values and scales, whatever is there, must not reach the sums
+            for (int r = 0; r < kGroup; ++r) {
+                if ((r & 15) < nl[r >> 4]) continue;
                 for (int j = lane; j < R::W / 4; j += 32) *reinterpret_cast<uint32_t*>(st + R::V + r * R::PITCH + j * 4) = 0;
                 if (lane < NB) st[R::VS + r * NB + lane] = 0;
             }
             __syncwarp();
         }
-        // S = K Q^T: this lane has keys g and g + 8 of queries 2t and 2t + 1
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        // S = K Q^T: this lane has keys g + 8r of queries 2t and 2t + 1
+        float s[4][2];
+        uint32_t ksw[4], vsw[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[r][0] = s[r][1] = 0.f;
+            ksw[r] = scale_word<NB>(st + R::KS, g + 8 * r);
+            vsw[r] = scale_word<NB>(st + R::VS, g + 8 * r);
+        }
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            uint32_t ka[4], kb[4];
-            const uint8_t* p = st + g * R::PITCH + (k * 32 + t * 8) * BITS / 8;
-            key_pairs<BITS>(p, ka);
-            key_pairs<BITS>(p + 8 * R::PITCH, kb);
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint32_t f0[4] = {ka[0], kb[0], ka[1], kb[1]}, f1[4] = {ka[2], kb[2], ka[3], kb[3]};
-            mma_f16(d, f0, q[k][0], q[k][1]);
-            mma_f16(d, f1, q[k][2], q[k][3]);
-            const float sa = scale_value(st[R::KS + g * NB + k]), sb = scale_value(st[R::KS + (g + 8) * NB + k]);
-            s[0] = fmaf(d[0], sa, s[0]);
-            s[1] = fmaf(d[1], sa, s[1]);
-            s[2] = fmaf(d[2], sb, s[2]);
-            s[3] = fmaf(d[3], sb, s[3]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t ka[4], kb[4];
+                const uint8_t* p = st + (g + 16 * h) * R::PITCH + (k * 32 + t * 8) * BITS / 8;
+                key_pairs<BITS>(p, ka);
+                key_pairs<BITS>(p + 8 * R::PITCH, kb);
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint32_t f0[4] = {ka[0], kb[0], ka[1], kb[1]}, f1[4] = {ka[2], kb[2], ka[3], kb[3]};
+                mma_f16(d, f0, q[k][0], q[k][1]);
+                mma_f16(d, f1, q[k][2], q[k][3]);
+                const float sa = word_scale(ksw[2 * h], k), sb = word_scale(ksw[2 * h + 1], k);
+                s[2 * h][0] = fmaf(d[0], sa, s[2 * h][0]);
+                s[2 * h][1] = fmaf(d[1], sa, s[2 * h][1]);
+                s[2 * h + 1][0] = fmaf(d[2], sb, s[2 * h + 1][0]);
+                s[2 * h + 1][1] = fmaf(d[3], sb, s[2 * h + 1][1]);
+            }
         }
-        s[0] = g < nl ? s[0] * c0 : -INFINITY;
-        s[1] = g < nl ? s[1] * c1 : -INFINITY;
-        s[2] = g + 8 < nl ? s[2] * c0 : -INFINITY;
-        s[3] = g + 8 < nl ? s[3] * c1 : -INFINITY;
-        const float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[r][0] *= c0;
+            s[r][1] *= c1;
+            if (!whole && g + 8 * (r & 1) >= nl[r >> 1]) s[r][0] = s[r][1] = -INFINITY;
+        }
+        const float t0 = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
+        const float t1 = fmaxf(fmaxf(s[0][1], s[1][1]), fmaxf(s[2][1], s[3][1]));
         if (__any_sync(0xffffffffu, t0 > m0 + 1.f || t1 > m1 + 1.f)) {
             float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
 #pragma unroll
@@ -400,34 +438,52 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             }
         }
         const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-        const float p[4] = {exp2f(s[0] - r0), exp2f(s[1] - r1), exp2f(s[2] - r0), exp2f(s[3] - r1)};
-        l0 += p[0] + p[2];
-        l1 += p[1] + p[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {                       // scores to weights
+            s[r][0] = exp2f(s[r][0] - r0);
+            s[r][1] = exp2f(s[r][1] - r1);
+            l0 += s[r][0];
+            l1 += s[r][1];
+        }
         // O += V^T P
+        // the group's largest value scales, of blocks 0, 2 and 1, 3 in the halves of two words
+        uint32_t top[2] = {0, 0};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            top[0] = __vmaxu2(top[0], vsw[r] & 0x00ff00ffu);
+            if (NB > 1) top[1] = __vmaxu2(top[1], (vsw[r] >> 8) & 0x00ff00ffu);
+        }
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+            top[0] = __vmaxu2(top[0], __shfl_xor_sync(0xffffffffu, top[0], w));
+            if (NB > 1) top[1] = __vmaxu2(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
+        }
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const uint32_t ea = st[R::VS + g * NB + k], eb = st[R::VS + (g + 8) * NB + k];
-            uint32_t top = max(ea, eb);
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, w));
-            // 2^14 * 2^(e - top), 0 below the smallest normal number
-            const float fa = __uint_as_float((uint32_t)max(141 + (int)ea - (int)top, 0) << 23);
-            const float fb = __uint_as_float((uint32_t)max(141 + (int)eb - (int)top, 0) << 23);
-            const uint32_t b0 = transpose8(pack_f16(p[0] * fa, p[1] * fa));
-            const uint32_t b1 = transpose8(pack_f16(p[2] * fb, p[3] * fb));
-            uint32_t va[4], vb[4];                          // keys 2t, 2t + 1 and 2t + 8, 2t + 9
-            const uint8_t* v = st + R::V + 2 * t * R::PITCH + (k * 32 + g * 4) * BITS / 8;
-            value_pairs<BITS>(v, v + R::PITCH, va);
-            value_pairs<BITS>(v + 8 * R::PITCH, v + 9 * R::PITCH, vb);
-            const float unit = scale_value(top) * 6.103515625e-05f;             // 2^-14
+            // weights times 2^14 over the largest scale (2^127 at most), the product times its inverse
+            const int tk = k < 2 ? top[k & 1] & 255 : top[k & 1] >> 16 & 255;
+            const float inv = __uint_as_float((uint32_t)min(254, 268 - tk) << 23);
+            const float unit = __uint_as_float(max(max(tk - 14, 0) << 23, 0x00400000));
+            float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t f[4] = {va[2 * h], va[2 * h + 1], vb[2 * h], vb[2 * h + 1]};
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(d, f, b0, b1);
+                const float fa = word_scale(vsw[2 * h], k) * inv, fb = word_scale(vsw[2 * h + 1], k) * inv;
+                const uint32_t b0 = transpose8(pack_f16(s[2 * h][0] * fa, s[2 * h][1] * fa));
+                const uint32_t b1 = transpose8(pack_f16(s[2 * h + 1][0] * fb, s[2 * h + 1][1] * fb));
+                uint32_t va[4], vb[4];                      // keys 2t, 2t + 1 and 2t + 8, 2t + 9 of the half
+                const uint8_t* v = st + R::V + (2 * t + 16 * h) * R::PITCH + (k * 32 + g * 4) * BITS / 8;
+                value_pairs<BITS>(v, v + R::PITCH, va);
+                value_pairs<BITS>(v + 8 * R::PITCH, v + 9 * R::PITCH, vb);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[2 * k + h][j] = fmaf(d[j], unit, o[2 * k + h][j]);
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t f[4] = {va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1]};
+                    mma_f16(d[e], f, b0, b1);
+                }
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[2 * k + e][j] = fmaf(d[e][j], unit, o[2 * k + e][j]);
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -489,6 +545,7 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
     __shared__ float red[2][HD / 32];
     const int h = blockIdx.x, b = blockIdx.y, e = threadIdx.x, warp = e >> 5, lane = e & 31;
     const float* base = a.ws + ((int64_t)b * a.heads + h) * a.splits * (2 + HD);
+    asm volatile("griddepcontrol.wait;" ::: "memory");      // the splits' states are written
     float mm = -INFINITY;
     for (int i = e; i < a.splits; i += HD) mm = fmaxf(mm, base[i * (2 + HD)]);
     mm = warp_max(mm);
@@ -515,15 +572,19 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
     a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(ll == 0.f ? 0.f : acc / ll);
 }
 
-// Splits of a sequence's keys: two rounds of the CTAs that fit the GPU (3 of 4 warps on each of 148
-// SMs), none with fewer than 128 keys of the longest sequence.
-int choose_splits(int batch, int heads, int kv_heads, int64_t longest) {
+// Keys of a split, the same for every sequence (the CTAs past a short one's end leave at once): two
+// rounds of the CTAs that fit the GPU (3 of 4 warps on each of 148 SMs) if every sequence were as
+// long as the longest may be, but at least 128, one group a warp; four rounds, for an even end,
+// where a split then still has 1024 keys.
+int keys_per_split(int batch, int heads, int kv_heads, int64_t longest) {
     const int group = heads / kv_heads;
     const int64_t ctas = (int64_t)batch * kv_heads * ((group + kQ - 1) / kQ);
-    const int64_t want = (6 * 148 + ctas - 1) / ctas, by_len = (longest + 127) / 128;
-    const int64_t s = want < by_len ? want : by_len;
-    return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+    const int64_t two = std::min(6 * 148 / ctas, (longest + 127) / 128), four = std::min(12 * 148 / ctas, longest / 1024);
+    const int64_t splits = std::min<int64_t>(std::max<int64_t>(std::max(two, four), 1), kMaxSplits);
+    constexpr int kStep = kWarps * kGroup;
+    return (int)(((longest + splits - 1) / splits + kStep - 1) / kStep * kStep);
 }
+int splits_of(int per, int64_t longest) { return (int)((longest + per - 1) / per); }
 
 constexpr int kMaxDevices = 64;
 
@@ -546,7 +607,21 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
     attend_kernel<HD, BITS><<<grid, kWarps * 32, bytes, s>>>(c, a);
     count_launches(1);
     if (a.splits > 1) {
-        combine_kernel<HD><<<dim3(a.heads, batch), HD, 0, s>>>(a);
+        // resident before the splits are done: the launch is hidden behind them
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(a.heads, batch);
+        cfg.blockDim = dim3(HD);
+        cfg.stream = s;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, combine_kernel<HD>, a);
+        if (e != cudaSuccess) {
+            record_cuda_error(e);
+            return VDIT_ERR_LAUNCH;
+        }
         count_launches(1);
     }
     return check_launch();
@@ -642,7 +717,9 @@ extern "C" int vdit_kv_cache_read(const void* kc, const void* vc, const void* k_
 extern "C" size_t vdit_attention_1q_cached_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads,
                                                            int32_t head_dim, int32_t max_pages, int32_t page_size) {
     if (batch < 1 || kv_heads < 1 || heads < kv_heads || head_dim < 1 || max_pages < 1 || page_size < 1) return 0;
-    const int splits = choose_splits(batch, heads, kv_heads, (int64_t)max_pages * page_size);
+    const int64_t longest = (int64_t)max_pages * page_size;
+    if (longest > INT32_MAX - 4096) return 0;
+    const int splits = splits_of(keys_per_split(batch, heads, kv_heads, longest), longest);
     return splits == 1 ? 0 : (size_t)batch * heads * splits * (2 + head_dim) * sizeof(float);
 }
 
@@ -659,15 +736,17 @@ extern "C" int vdit_attention_1q_cached(const void* q, int64_t ldq, const void* 
     if (!q || !page_table || !lengths || !out || batch < 0 || heads < 1 || heads % kv_heads || max_pages < 1 ||
         ld_table < 0 || ldq < (int64_t)heads * head_dim || ldo < (int64_t)heads * head_dim)
         return VDIT_ERR_ARG;
-    if (batch > 65535 || heads > 65535) return VDIT_ERR_UNSUPPORTED;
+    if (batch > 65535 || heads > 65535 || (int64_t)max_pages * page_size > INT32_MAX - 4096)
+        return VDIT_ERR_UNSUPPORTED;
     if (!aligned16(q) || ldq % 8) return VDIT_ERR_ALIGN;
     if (batch == 0) return VDIT_OK;
-    const int splits = choose_splits(batch, heads, kv_heads, (int64_t)max_pages * page_size);
+    const int64_t longest = (int64_t)max_pages * page_size;
+    const int per = keys_per_split(batch, heads, kv_heads, longest), splits = splits_of(per, longest);
     if (workspace_bytes < vdit_attention_1q_cached_workspace_bytes(batch, heads, kv_heads, head_dim, max_pages, page_size) ||
         (splits > 1 && !workspace))
         return VDIT_ERR_WORKSPACE;
     const AttnArgs a{static_cast<const __nv_bfloat16*>(q), ldq, static_cast<__nv_bfloat16*>(out), ldo, page_table,
-                     ld_table, lengths, max_pages, heads, heads / kv_heads, splits,
+                     ld_table, lengths, max_pages, heads, heads / kv_heads, splits, per,
                      softmax_scale * 1.4426950408889634f, static_cast<float*>(workspace)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     auto run = [&](auto hd) {
