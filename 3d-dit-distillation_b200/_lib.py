@@ -17,6 +17,13 @@ LIB_PATH = Path(__file__).resolve().parent / "libvdit.so"
 _c_i32, _c_i64, _c_f32, _c_f64, _c_sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
 _vp = ctypes.c_void_p
 
+
+class KvCacheStruct(ctypes.Structure):
+    """``vdit_kv_cache`` of include/vdit.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scales", _vp), ("v_scales", _vp), ("pages", _c_i64),
+                ("page_size", _c_i32), ("heads", _c_i32), ("head_dim", _c_i32), ("bits", _c_i32)]
+
+
 # name -> (restype, argtypes), mirrors include/vdit.h
 SIGNATURES = {
     "vdit_version": (ctypes.c_char_p, []),
@@ -67,14 +74,11 @@ SIGNATURES = {
     "vdit_mxfp4_quantize": (ctypes.c_int, [_vp, _c_i32, _c_i64, _c_i64, _c_i32, _vp, _vp, _vp]),
     "vdit_mxfp4_dequantize": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i32, _vp, _c_i32, _c_i64, _vp]),
     "vdit_linear_mxfp4": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp]),
-    "vdit_kv_cache_write": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i32,
-                                           _c_i32, _c_i32, _c_i32, _vp]),
-    "vdit_kv_cache_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp, _c_i64, _vp,
-                                          _c_i64, _vp, _c_i64, _c_i32, _vp]),
+    "vdit_kv_cache_write": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp]),
+    "vdit_kv_cache_read": (ctypes.c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i32, _vp]),
     "vdit_attention_1q_cached_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
-    "vdit_attention_1q_cached": (ctypes.c_int, [_vp, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32,
-                                                _c_i32, _vp, _c_i64, _c_i32, _vp, _c_i32, _c_i32, _c_f32, _vp, _c_i64,
-                                                _vp, _c_sz, _vp]),
+    "vdit_attention_1q_cached": (ctypes.c_int, [_vp, _c_i64, _vp, _vp, _c_i64, _c_i32, _vp, _c_i32, _c_i32, _c_f32,
+                                                _vp, _c_i64, _vp, _c_sz, _vp]),
     "vdit_gather_rows_f32": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i32, _vp, _vp]),
     "vdit_cfg_reuse_workspace_bytes": (_c_sz, []),
     "vdit_cfg_reuse_euler": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_f32, _c_f32, _c_f32, _c_f32, _c_f32, _c_i32,

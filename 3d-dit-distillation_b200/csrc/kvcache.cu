@@ -25,6 +25,7 @@ using namespace mx;
 constexpr int kErrIndex = 0x4B56;   // "KV": a slot, page or length outside the cache
 constexpr int kThreads = 256;
 constexpr int kMaxSplits = 1024;
+constexpr int64_t kMaxKeys = INT32_MAX - (1 << 20);          // of one sequence: positions stay int32
 
 struct Cache {
     uint8_t *k, *v, *ks, *vs;
@@ -142,9 +143,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 // queries a key head), so both products run on mma.sync m16n8k16: a pair of elements is one
 // conversion to f16 (exact for both element types) and up to 8 queries of a key head share it.
 //
-// A CTA takes one sequence, one key head, up to 8 of its queries and one range ("split") of the keys.
-// Its warps are independent until the end: each takes every fourth group of 32 consecutive keys (two
-// halves of 16, each in one page), copied by cp.async into the warp's own ring, rows padded to an odd
+// A CTA takes one sequence, one key head, up to 8 of its queries and a share ("split") of the keys.
+// Its warps are independent until the end: each takes groups of 32 consecutive keys (two halves of
+// 16, each in one page), copied by cp.async into the warp's own ring, rows padded to an odd
 // number of 16-byte chunks so that the fragment reads spread over the banks.  Per group and
 // 32-channel block:
 //   S = K Q^T   32 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
@@ -170,7 +171,8 @@ struct AttnArgs {
     const int32_t* lengths;                  // [batch]
     int max_pages;                           // entries of a table row
     int heads, group;                        // query heads, and how many share a key head
-    int splits, per;                         // key ranges, and keys of each
+    int splits;                              // key ranges of a sequence
+    int cluster;                             // CTAs of a cluster: 1, or all splits of a sequence and head
     float scale_log2;
     float* ws;                               // [batch, heads, splits, 2 + hd] when splits > 1
 };
@@ -183,6 +185,13 @@ __device__ __forceinline__ int64_t length_of(const AttnArgs& a, int page_size, i
         return n < 0 ? 0 : most;
     }
     return n;
+}
+
+// a float of shared memory at the same place in CTA `rank` of the cluster
+__device__ __forceinline__ float load_cluster(uint32_t addr, int rank) {
+    float x;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::mapa_shared(addr, rank)));
+    return x;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -274,15 +283,19 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     using R = Ring<HD, BITS>;
     constexpr int NB = R::NB, kStages = R::STAGES;
     extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float joined[kQ][2];                         // max and sum of the CTA's queries
     __shared__ int live[kWarps][kStages][2];                // keys that count of the halves of a group
     const int split = blockIdx.x, chunks = (a.group + kQ - 1) / kQ;
     const int kh = blockIdx.y / chunks, q0 = (blockIdx.y % chunks) * kQ, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nq = min(kQ, a.group - q0);
     asm volatile("griddepcontrol.launch_dependents;");
-    constexpr int kStep = kWarps * kGroup;
-    const int len = (int)length_of(a, c.page_size, b);      // as int32 as the caller's
-    const int k0 = (int)min((int64_t)len, (int64_t)split * a.per), k1 = (int)min((int64_t)len, (int64_t)k0 + a.per);
+    constexpr int step = kWarps * kGroup;
+    const int len = (int)length_of(a, c.page_size, b);      // an int32, as the caller's
+    const int per = ((len + kGroup - 1) / kGroup + a.splits - 1) / a.splits * kGroup;
+    const int first = (int)min((int64_t)len, (int64_t)split * per) + warp * kGroup;   // groups at first + i * step ...
+    const int end = (int)min((int64_t)len, (int64_t)(split + 1) * per);               // ... below end
+    const int mine = first < end ? (end - first + step - 1) / step : 0;
 
     // query g of this lane as the B fragments of S: per block four f16 pairs of channels t * 8 ...
     uint32_t q[NB][4];
@@ -312,24 +325,22 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     }
 
     uint8_t* ring = smem + warp * R::WARP;
-    const int first = k0 + warp * kGroup;                   // this warp's groups start at first + i * kStep
-    const int mine = first < k1 ? (k1 - first + kStep - 1) / kStep : 0;
     const int32_t* table = a.table + b * a.ldt;
     int pages = -1;                                         // lane j: page of half j of 16 groups
     auto issue = [&](int i, int s) {                        // copy group i of this warp, if there is one, to stage s
         if (i < mine) {
             if ((i & 15) == 0) {
-                const int j = first + (i + (lane >> 1)) * kStep + (lane & 1) * 16;
-                pages = j < k1 ? __ldg(table + (j >> c.page_shift)) : -1;
+                const int j = first + (i + (lane >> 1)) * step + (lane & 1) * 16;
+                pages = j < end ? __ldg(table + (j >> c.page_shift)) : -1;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int page = __shfl_sync(0xffffffffu, pages, (i & 15) * 2 + h);
-                const int key = first + i * kStep + h * 16;
-                const bool there = key < k1 && page >= 0 && page < c.pages;
+                const int key = first + i * step + h * 16;
+                const bool there = key < end && page >= 0 && page < c.pages;
                 if (lane == 0) {
-                    live[warp][s][h] = there ? min(16, k1 - key) : 0;
-                    if (key < k1 && !there) atomicExch(&g_kvcache_error, kErrIndex);
+                    live[warp][s][h] = there ? min(16, end - key) : 0;
+                    if (key < end && !there) atomicExch(&g_kvcache_error, kErrIndex);
                 }
                 if (!there) continue;
                 const int64_t row = ((int64_t)page * c.heads + kh) * c.page_size + (key & (c.page_size - 1));
@@ -527,15 +538,41 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         const int h = kh * a.group + q0 + j;
         if (a.splits == 1) {
             a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(ll == 0.f ? 0.f : acc / ll);
-        } else {
+        } else if (a.cluster == 1) {
             float* x = a.ws + (((int64_t)b * a.heads + h) * a.splits + split) * (2 + HD);
             x[2 + e] = acc;
             if (e == 0) {
                 x[0] = mm;
                 x[1] = ll;
             }
+        } else {
+            so[j * HD + e] = acc;                           // in warp 0's place, which no other thread reads
+            if (e == 0) {
+                joined[j][0] = mm;
+                joined[j][1] = ll;
+            }
         }
     }
+    if (a.cluster == 1) return;
+    // the splits of a sequence and head are the CTAs of this cluster: each joins its part of the
+    // outputs through distributed shared memory
+    tc::cluster_sync();
+    const uint32_t so_at = tc::smem_u32(so), joined_at = tc::smem_u32(joined);
+    for (int i = split * kWarps * 32 + threadIdx.x; i < nq * HD; i += a.cluster * kWarps * 32) {
+        const int j = i / HD;
+        float mm = -INFINITY;
+        for (int r = 0; r < a.cluster; ++r) mm = fmaxf(mm, load_cluster(joined_at + j * 8, r));
+        float acc = 0.f, ll = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < a.cluster; ++r) {
+            const float mr = load_cluster(joined_at + j * 8, r);
+            const float f = mr == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : exp2f(mr - mm);
+            acc = fmaf(load_cluster(so_at + i * 4, r), f, acc);
+            ll = fmaf(load_cluster(joined_at + j * 8 + 4, r), f, ll);
+        }
+        a.out[b * a.ldo + (int64_t)(kh * a.group + q0) * HD + i] = f2bf(ll == 0.f ? 0.f : acc / ll);
+    }
+    tc::cluster_sync();                                     // no CTA leaves while another reads its memory
 }
 
 // joins the splits of one (sequence, head); no keys give zeros
@@ -572,51 +609,69 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
     a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(ll == 0.f ? 0.f : acc / ll);
 }
 
-// Keys of a split, the same for every sequence (the CTAs past a short one's end leave at once): two
-// rounds of the CTAs that fit the GPU (3 of 4 warps on each of 148 SMs) if every sequence were as
-// long as the longest may be, but at least 128, one group a warp; four rounds, for an even end,
-// where a split then still has 1024 keys.
-int keys_per_split(int batch, int heads, int kv_heads, int64_t longest) {
+// How the keys of a sequence are split: two rounds of the CTAs that fit the GPU (3 of 4 warps on each
+// of 148 SMs) but no fewer than 128 keys of the longest sequence, one group a warp; four rounds,
+// for an even end, where a split then still has 1024.  Where up to 16 splits that all run at once have
+// no more than 2048 keys each, they are a cluster, which joins them itself (one launch, no workspace);
+// otherwise their states go through the workspace to a second kernel (16 sequences of up to 32768
+// keys: 200 us, in clusters of 2 or 8 272 and 233).
+struct Plan {
+    int splits, cluster;
+};
+Plan plan_of(int batch, int heads, int kv_heads, int64_t longest) {
     const int group = heads / kv_heads;
     const int64_t ctas = (int64_t)batch * kv_heads * ((group + kQ - 1) / kQ);
     const int64_t two = std::min(6 * 148 / ctas, (longest + 127) / 128), four = std::min(12 * 148 / ctas, longest / 1024);
-    const int64_t splits = std::min<int64_t>(std::max<int64_t>(std::max(two, four), 1), kMaxSplits);
-    constexpr int kStep = kWarps * kGroup;
-    return (int)(((longest + splits - 1) / splits + kStep - 1) / kStep * kStep);
+    const int64_t want = std::min<int64_t>(std::max<int64_t>(std::max(two, four), 1), kMaxSplits);
+    int c = 1;
+    while (c < 16 && c < want && ctas * 2 * c <= 4 * 148) c *= 2;
+    if (c >= want || (longest <= (int64_t)c * 2048 && ctas * c >= 148)) return {c, c};
+    return {(int)want, 1};
 }
-int splits_of(int per, int64_t longest) { return (int)((longest + per - 1) / per); }
 
 constexpr int kMaxDevices = 64;
 
 template <int HD, int BITS>
 int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) {
-    static std::atomic<bool> ready[kMaxDevices];            // the kernel's shared memory size is set, per device
+    static std::atomic<bool> ready[kMaxDevices];            // the kernel's attributes are set, per device
     constexpr int bytes = Ring<HD, BITS>::BYTES;
     int dev = -1;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) return VDIT_ERR_UNSUPPORTED;
-    if (e == cudaSuccess && bytes > 48 * 1024 && !ready[dev].load(std::memory_order_acquire)) {
+    if (e == cudaSuccess && !ready[dev].load(std::memory_order_acquire)) {
         e = cudaFuncSetAttribute(attend_kernel<HD, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(attend_kernel<HD, BITS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) ready[dev].store(true, std::memory_order_release);
     }
     if (e != cudaSuccess) {
         record_cuda_error(e);
         return VDIT_ERR_LAUNCH;
     }
-    const dim3 grid(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
-    attend_kernel<HD, BITS><<<grid, kWarps * 32, bytes, s>>>(c, a);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attend_kernel<HD, BITS>, c, a);
+    if (e != cudaSuccess) {
+        record_cuda_error(e);
+        return VDIT_ERR_LAUNCH;
+    }
     count_launches(1);
-    if (a.splits > 1) {
+    if (a.splits > a.cluster) {
         // resident before the splits are done: the launch is hidden behind them
-        cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(a.heads, batch);
         cfg.blockDim = dim3(HD);
-        cfg.stream = s;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.dynamicSmemBytes = 0;
         e = cudaLaunchKernelEx(&cfg, combine_kernel<HD>, a);
         if (e != cudaSuccess) {
             record_cuda_error(e);
@@ -628,17 +683,18 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
 }
 
 // the cache's own checks; fills c
-int check_cache(void* k, void* v, void* ks, void* vs, int64_t pages, int32_t page_size, int32_t heads, int32_t hd,
-                int32_t bits, Cache* c) {
-    if (!k || !v || !ks || !vs || pages < 1 || page_size < 1 || heads < 1 || hd < 1) return VDIT_ERR_ARG;
-    if ((bits != 4 && bits != 8) || hd % 32 || hd > 128 || (page_size & (page_size - 1)) || page_size < 16 || page_size > 1024 ||
-        heads > 4096 || pages > INT32_MAX)
+int check_cache(const vdit_kv_cache* v, Cache* c) {
+    if (!v || !v->k || !v->v || !v->k_scales || !v->v_scales || v->pages < 1 || v->page_size < 1 || v->heads < 1 ||
+        v->head_dim < 1)
+        return VDIT_ERR_ARG;
+    if ((v->bits != 4 && v->bits != 8) || v->head_dim % 32 || v->head_dim > 128 || (v->page_size & (v->page_size - 1)) ||
+        v->page_size < 16 || v->page_size > 1024 || v->heads > 4096 || v->pages > INT32_MAX)
         return VDIT_ERR_UNSUPPORTED;
-    if (!aligned16(k) || !aligned16(v) || !aligned16(ks) || !aligned16(vs)) return VDIT_ERR_ALIGN;
+    if (!aligned16(v->k) || !aligned16(v->v) || !aligned16(v->k_scales) || !aligned16(v->v_scales)) return VDIT_ERR_ALIGN;
     int shift = 0;
-    while ((1 << shift) < page_size) ++shift;
-    *c = Cache{static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), static_cast<uint8_t*>(ks), static_cast<uint8_t*>(vs),
-               pages, page_size, shift, heads, hd};
+    while ((1 << shift) < v->page_size) ++shift;
+    *c = Cache{static_cast<uint8_t*>(v->k), static_cast<uint8_t*>(v->v), static_cast<uint8_t*>(v->k_scales),
+               static_cast<uint8_t*>(v->v_scales), v->pages, v->page_size, shift, v->heads, v->head_dim};
     return VDIT_OK;
 }
 
@@ -668,13 +724,12 @@ using namespace vdit;
 using namespace vdit::kv;
 
 extern "C" int vdit_kv_cache_write(const void* k, int64_t ldk, const void* v, int64_t ldv, const int64_t* slots,
-                                   int64_t n, void* kc, void* vc, void* k_scales, void* v_scales, int64_t pages,
-                                   int32_t page_size, int32_t heads, int32_t head_dim, int32_t bits,
-                                   vdit_stream_t stream) {
+                                   int64_t n, const vdit_kv_cache* cache, vdit_stream_t stream) {
     Cache c;
-    const int rc = check_cache(kc, vc, k_scales, v_scales, pages, page_size, heads, head_dim, bits, &c);
+    const int rc = check_cache(cache, &c);
     if (rc != VDIT_OK) return rc;
-    if (!k || !v || !slots || n < 0 || ldk < heads * head_dim || ldv < heads * head_dim) return VDIT_ERR_ARG;
+    const int d = c.heads * c.hd;
+    if (!k || !v || !slots || n < 0 || ldk < d || ldv < d) return VDIT_ERR_ARG;
     if (!aligned16(k) || !aligned16(v) || ldk % 8 || ldv % 8) return VDIT_ERR_ALIGN;
     if (n == 0) return VDIT_OK;
     const int64_t blocks = row_blocks(c, n);
@@ -682,21 +737,19 @@ extern "C" int vdit_kv_cache_write(const void* k, int64_t ldk, const void* v, in
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const auto* kp = static_cast<const __nv_bfloat16*>(k);
     const auto* vp = static_cast<const __nv_bfloat16*>(v);
-    if (bits == 4) write_kernel<4><<<(unsigned)blocks, kThreads, 0, s>>>(kp, ldk, vp, ldv, slots, n, c);
+    if (cache->bits == 4) write_kernel<4><<<(unsigned)blocks, kThreads, 0, s>>>(kp, ldk, vp, ldv, slots, n, c);
     else write_kernel<8><<<(unsigned)blocks, kThreads, 0, s>>>(kp, ldk, vp, ldv, slots, n, c);
     count_launches(1);
     return check_launch();
 }
 
-extern "C" int vdit_kv_cache_read(const void* kc, const void* vc, const void* k_scales, const void* v_scales,
-                                  int64_t pages, int32_t page_size, int32_t heads, int32_t head_dim, int32_t bits,
-                                  const int64_t* slots, int64_t n, void* k, int64_t ldk, void* v, int64_t ldv,
-                                  int32_t out_type, vdit_stream_t stream) {
+extern "C" int vdit_kv_cache_read(const vdit_kv_cache* cache, const int64_t* slots, int64_t n, void* k, int64_t ldk,
+                                  void* v, int64_t ldv, int32_t out_type, vdit_stream_t stream) {
     Cache c;
-    const int rc = check_cache(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(k_scales),
-                               const_cast<void*>(v_scales), pages, page_size, heads, head_dim, bits, &c);
+    const int rc = check_cache(cache, &c);
     if (rc != VDIT_OK) return rc;
-    if (!k || !v || !slots || n < 0 || ldk < heads * head_dim || ldv < heads * head_dim) return VDIT_ERR_ARG;
+    const int d = c.heads * c.hd;
+    if (!k || !v || !slots || n < 0 || ldk < d || ldv < d) return VDIT_ERR_ARG;
     if (out_type != VDIT_BF16 && out_type != VDIT_F32) return VDIT_ERR_ARG;
     const int per16 = out_type == VDIT_F32 ? 4 : 8;
     if (!aligned16(k) || !aligned16(v) || ldk % per16 || ldv % per16) return VDIT_ERR_ALIGN;
@@ -705,7 +758,7 @@ extern "C" int vdit_kv_cache_read(const void* kc, const void* vc, const void* k_
     if (!blocks) return VDIT_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     auto run = [&](auto* kp, auto* vp) {
-        if (bits == 4) read_kernel<4><<<(unsigned)blocks, kThreads, 0, s>>>(c, slots, n, kp, ldk, vp, ldv);
+        if (cache->bits == 4) read_kernel<4><<<(unsigned)blocks, kThreads, 0, s>>>(c, slots, n, kp, ldk, vp, ldv);
         else read_kernel<8><<<(unsigned)blocks, kThreads, 0, s>>>(c, slots, n, kp, ldk, vp, ldv);
     };
     if (out_type == VDIT_F32) run(static_cast<float*>(k), static_cast<float*>(v));
@@ -718,40 +771,39 @@ extern "C" size_t vdit_attention_1q_cached_workspace_bytes(int32_t batch, int32_
                                                            int32_t head_dim, int32_t max_pages, int32_t page_size) {
     if (batch < 1 || kv_heads < 1 || heads < kv_heads || head_dim < 1 || max_pages < 1 || page_size < 1) return 0;
     const int64_t longest = (int64_t)max_pages * page_size;
-    if (longest > INT32_MAX - 4096) return 0;
-    const int splits = splits_of(keys_per_split(batch, heads, kv_heads, longest), longest);
-    return splits == 1 ? 0 : (size_t)batch * heads * splits * (2 + head_dim) * sizeof(float);
+    if (longest > kMaxKeys) return 0;
+    const Plan plan = plan_of(batch, heads, kv_heads, longest);
+    return plan.splits == plan.cluster ? 0 : (size_t)batch * heads * plan.splits * (2 + head_dim) * sizeof(float);
 }
 
-extern "C" int vdit_attention_1q_cached(const void* q, int64_t ldq, const void* kc, const void* vc,
-                                        const void* k_scales, const void* v_scales, int64_t pages, int32_t page_size,
-                                        int32_t kv_heads, int32_t head_dim, int32_t bits, const int32_t* page_table,
-                                        int64_t ld_table, int32_t max_pages, const int32_t* lengths, int32_t batch,
-                                        int32_t heads, float softmax_scale, void* out, int64_t ldo, void* workspace,
-                                        size_t workspace_bytes, vdit_stream_t stream) {
+extern "C" int vdit_attention_1q_cached(const void* q, int64_t ldq, const vdit_kv_cache* cache,
+                                        const int32_t* page_table, int64_t ld_table, int32_t max_pages,
+                                        const int32_t* lengths, int32_t batch, int32_t heads, float softmax_scale,
+                                        void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                                        vdit_stream_t stream) {
     Cache c;
-    const int rc = check_cache(const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(k_scales),
-                               const_cast<void*>(v_scales), pages, page_size, kv_heads, head_dim, bits, &c);
+    const int rc = check_cache(cache, &c);
     if (rc != VDIT_OK) return rc;
+    const int kv_heads = c.heads, head_dim = c.hd, page_size = c.page_size;
     if (!q || !page_table || !lengths || !out || batch < 0 || heads < 1 || heads % kv_heads || max_pages < 1 ||
         ld_table < 0 || ldq < (int64_t)heads * head_dim || ldo < (int64_t)heads * head_dim)
         return VDIT_ERR_ARG;
-    if (batch > 65535 || heads > 65535 || (int64_t)max_pages * page_size > INT32_MAX - 4096)
+    if (batch > 65535 || heads > 65535 || (int64_t)max_pages * page_size > kMaxKeys)
         return VDIT_ERR_UNSUPPORTED;
     if (!aligned16(q) || ldq % 8) return VDIT_ERR_ALIGN;
     if (batch == 0) return VDIT_OK;
     const int64_t longest = (int64_t)max_pages * page_size;
-    const int per = keys_per_split(batch, heads, kv_heads, longest), splits = splits_of(per, longest);
+    const Plan plan = plan_of(batch, heads, kv_heads, longest);
     if (workspace_bytes < vdit_attention_1q_cached_workspace_bytes(batch, heads, kv_heads, head_dim, max_pages, page_size) ||
-        (splits > 1 && !workspace))
+        (plan.splits > plan.cluster && !workspace))
         return VDIT_ERR_WORKSPACE;
     const AttnArgs a{static_cast<const __nv_bfloat16*>(q), ldq, static_cast<__nv_bfloat16*>(out), ldo, page_table,
-                     ld_table, lengths, max_pages, heads, heads / kv_heads, splits, per,
+                     ld_table, lengths, max_pages, heads, heads / kv_heads, plan.splits, plan.cluster,
                      softmax_scale * 1.4426950408889634f, static_cast<float*>(workspace)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     auto run = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        return bits == 4 ? launch_attend<HD, 4>(c, a, batch, s) : launch_attend<HD, 8>(c, a, batch, s);
+        return cache->bits == 4 ? launch_attend<HD, 4>(c, a, batch, s) : launch_attend<HD, 8>(c, a, batch, s);
     };
     if (head_dim == 32) return run(std::integral_constant<int, 32>{});
     if (head_dim == 64) return run(std::integral_constant<int, 64>{});

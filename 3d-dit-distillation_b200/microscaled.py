@@ -9,13 +9,14 @@ it computes in bf16.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
 
-from ._lib import check, lib, ptr
+from ._lib import KvCacheStruct, check, lib, ptr
 
 BF16 = torch.bfloat16
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}     # VDIT_BF16, VDIT_F16, VDIT_F32
@@ -198,8 +199,9 @@ class MxKvCache:
         self._k, self._v = (torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8, device=device) for _ in range(2))
         self._ks, self._vs = (torch.zeros(*shape, head_dim // BLOCK, dtype=torch.uint8, device=device) for _ in range(2))
         self.device = self._k.device
-        self._buffers = tuple(t.data_ptr() for t in (self._k, self._v, self._ks, self._vs))
-        self._geometry = (pages, page_size, kv_heads, head_dim, bits)
+        self._struct = KvCacheStruct(*(t.data_ptr() for t in (self._k, self._v, self._ks, self._vs)), pages, page_size,
+                                     kv_heads, head_dim, bits)
+        self._ref = ctypes.addressof(self._struct)
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -231,8 +233,8 @@ def kv_cache_write(cache: MxKvCache, k: torch.Tensor, v: torch.Tensor, slots: to
     if _elsewhere(k):
         with torch.cuda.device(cache.device):
             return kv_cache_write(cache, k, v, slots)
-    check(lib().vdit_kv_cache_write(pk, ldk, v.data_ptr(), ldv, slots.data_ptr(), n, *cache._buffers,
-                                    *cache._geometry, _stream(cache.device.index)), "kv_cache_write")
+    check(lib().vdit_kv_cache_write(pk, ldk, v.data_ptr(), ldv, slots.data_ptr(), n, cache._ref,
+                                    _stream(cache.device.index)), "kv_cache_write")
 
 
 def kv_cache_read(cache: MxKvCache, slots: torch.Tensor, dtype: torch.dtype = BF16) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -250,7 +252,7 @@ def kv_cache_read(cache: MxKvCache, slots: torch.Tensor, dtype: torch.dtype = BF
     k = torch.empty((n, d), dtype=dtype, device=dev)
     v = torch.empty((n, d), dtype=dtype, device=dev)
     if n:
-        check(lib().vdit_kv_cache_read(*cache._buffers, *cache._geometry, ps, n, k.data_ptr(), d, v.data_ptr(), d,
+        check(lib().vdit_kv_cache_read(cache._ref, ps, n, k.data_ptr(), d, v.data_ptr(), d,
                                        _TYPES[dtype], _stream(dev.index)), "kv_cache_read")
     return k, v
 
@@ -291,7 +293,7 @@ def attention_1q_cached(q: torch.Tensor, cache: MxKvCache, page_table: torch.Ten
         heads = d // hd
         nb = _attend_workspace(b, heads, cache.kv_heads, hd, pages, cache.page_size)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        check(lib().vdit_attention_1q_cached(pq, ldq, *cache._buffers, *cache._geometry, page_table.data_ptr(),
+        check(lib().vdit_attention_1q_cached(pq, ldq, cache._ref, page_table.data_ptr(),
                                              page_table.stride(0) if b > 1 else pages, pages, lengths.data_ptr(), b,
                                              heads, 1.0 / math.sqrt(hd) if scale is None else float(scale),
                                              out.data_ptr(), d, None if ws is None else ws.data_ptr(), nb,

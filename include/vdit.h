@@ -348,40 +348,41 @@ int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, const void* w_c
 
 /* ------------------------------------------------------------------ key/value cache */
 /* A paged cache of keys and values in a microscaled format, bits 8 (e4m3) or 4 (e2m1).  Slot
- * page * page_size + offset holds one row of heads * head_dim channels: kc and vc are
+ * page * page_size + offset holds one row of heads * head_dim channels: k and v are
  * [pages, heads, page_size, head_dim * bits / 8] bytes, k_scales and v_scales
- * [pages, heads, page_size, head_dim / 32] bytes.  page_size is a power of two from 16 to
- * 1024; head_dim 32, 64, 96 or 128; all four buffers 16-byte aligned.
- *
- * write: rows k, v bf16 [n, ldk], [n, ldv] are quantised into slots[n]; a negative slot is
+ * [pages, heads, page_size, head_dim / 32] bytes, device memory of the caller's, 16-byte aligned.
+ * page_size is a power of two from 16 to 1024; head_dim 32, 64, 96 or 128.  The struct itself is
+ * host memory, read during the call. */
+typedef struct vdit_kv_cache {
+    void *k, *v, *k_scales, *v_scales;
+    int64_t pages;
+    int32_t page_size, heads, head_dim, bits;
+} vdit_kv_cache;
+
+/* write: rows k, v bf16 [n, ldk], [n, ldv] are quantised into slots[n]; a negative slot is
  * skipped, and no slot may appear twice among the others.  read: the rows the slots stand for, bf16
  * or fp32; a negative slot gives zeros.  A slot past the cache is left out (read: zeros) and
  * recorded in the device error word. */
 int vdit_kv_cache_write(const void* k, int64_t ldk, const void* v, int64_t ldv, const int64_t* slots, int64_t n,
-                        void* kc, void* vc, void* k_scales, void* v_scales, int64_t pages, int32_t page_size,
-                        int32_t heads, int32_t head_dim, int32_t bits, vdit_stream_t stream);
-int vdit_kv_cache_read(const void* kc, const void* vc, const void* k_scales, const void* v_scales, int64_t pages,
-                       int32_t page_size, int32_t heads, int32_t head_dim, int32_t bits, const int64_t* slots,
-                       int64_t n, void* k, int64_t ldk, void* v, int64_t ldv, int32_t out_type,
-                       vdit_stream_t stream);
+                        const vdit_kv_cache* cache, vdit_stream_t stream);
+int vdit_kv_cache_read(const vdit_kv_cache* cache, const int64_t* slots, int64_t n, void* k, int64_t ldk, void* v,
+                       int64_t ldv, int32_t out_type, vdit_stream_t stream);
 
 /* One query per sequence and head over cached keys: vdit_attention_1q for a batch, reading the
  * cache.  Sequence b attends to its first lengths[b] (int32) keys, key i in page
  * page_table[b * ld_table + i / page_size] (int32) at offset i % page_size; entries past its
- * length are not read (ld_table 0: every sequence has the same pages).  No keys give zeros.  q bf16 [batch, ldq] and out bf16 [batch, ldo] hold
- * heads * head_dim channels a row; query head h reads key head h / (heads / kv_heads).  A page
- * outside the cache is left out and a length outside [0, max_pages * page_size] is clipped to it,
- * both recorded in the device error word.  Partial states of split key ranges go to the
- * caller's workspace (of vdit_attention_1q_cached_workspace_bytes bytes, 16-byte aligned; may be
- * 0). */
+ * length are not read (ld_table 0: every sequence has the same pages).  No keys give zeros.  q bf16
+ * [batch, ldq] and out bf16 [batch, ldo] hold heads * head_dim channels a row; query head h reads key
+ * head h / (heads / cache->heads).  A page outside the cache is left out and a length outside
+ * [0, max_pages * page_size] is clipped to it, both recorded in the device error word.  Partial
+ * states of split keys may go to the caller's workspace (of vdit_attention_1q_cached_workspace_bytes
+ * bytes, 16-byte aligned; may be 0). */
 size_t vdit_attention_1q_cached_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                                 int32_t max_pages, int32_t page_size);
-int vdit_attention_1q_cached(const void* q, int64_t ldq, const void* kc, const void* vc, const void* k_scales,
-                             const void* v_scales, int64_t pages, int32_t page_size, int32_t kv_heads,
-                             int32_t head_dim, int32_t bits, const int32_t* page_table, int64_t ld_table,
-                             int32_t max_pages, const int32_t* lengths, int32_t batch, int32_t heads,
-                             float softmax_scale, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
-                             vdit_stream_t stream);
+int vdit_attention_1q_cached(const void* q, int64_t ldq, const vdit_kv_cache* cache, const int32_t* page_table,
+                             int64_t ld_table, int32_t max_pages, const int32_t* lengths, int32_t batch,
+                             int32_t heads, float softmax_scale, void* out, int64_t ldo, void* workspace,
+                             size_t workspace_bytes, vdit_stream_t stream);
 
 /* ------------------------------------------------------------------ sampler glue */
 /* dst[j,:] = src[idx[j],:] for fp32 rows of width c (noise[perm], lib/fast_flow.py:2576). */

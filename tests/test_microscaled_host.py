@@ -1,5 +1,7 @@
 """CPU tests of the low-bit operators: the 64-bit restatement itself, the refusals of the wrappers
 and of the C entry points, and the addresses the cache kernels form."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -92,20 +94,31 @@ def test_c_entry_points_check_before_any_launch():
     assert lib.vdit_linear_mxfp4(16, 16, 16, 16, None, 16, 56, 4, 64, 64, None) == -1
     assert lib.vdit_linear_mxfp4(16, 16, 8, 16, None, 16, 64, 4, 64, 64, None) == -2
     assert lib.vdit_linear_mxfp4(16, 16, 16, 16, None, 16, 64, 0, 64, 64, None) == 0
-    assert lib.vdit_kv_cache_write(16, 64, 16, 64, 16, 3, 16, 16, 16, 16, 2, 24, 1, 64, 8, None) == -4
-    assert lib.vdit_kv_cache_write(16, 64, 16, 64, 16, 3, 16, 16, 16, 16, 2, 16, 1, 48, 8, None) == -4
-    assert lib.vdit_kv_cache_write(16, 56, 16, 64, 16, 3, 16, 16, 16, 16, 2, 16, 1, 64, 8, None) == -1
-    assert lib.vdit_kv_cache_write(16, 64, 16, 64, 16, 0, 16, 16, 16, 16, 2, 16, 1, 64, 8, None) == 0
-    assert lib.vdit_kv_cache_read(16, 16, 16, 16, 2, 16, 1, 64, 8, 16, 3, 16, 64, 16, 64, 1, None) == -1
-    args = [16, 128, 16, 16, 16, 16, 2, 16, 2, 64, 8, 16, 4, 4, 16, 1, 2, 0.125, 16, 128, None, 0, None]
-    need = lib.vdit_attention_1q_cached_workspace_bytes(1, 2, 2, 64, 64, 16)
+
+    def cache(**kw):
+        a = dict(k=16, v=16, k_scales=16, v_scales=16, pages=2, page_size=16, heads=2, head_dim=64, bits=8)
+        a.update(kw)
+        return ctypes.byref(_lib.KvCacheStruct(**a))
+
+    for kw, rc in ((dict(page_size=24), -4), (dict(page_size=8), -4), (dict(head_dim=48), -4), (dict(bits=5), -4),
+                   (dict(k=None), -1), (dict(pages=0), -1), (dict(v_scales=8), -2), (dict(v=24), -2)):
+        assert lib.vdit_kv_cache_write(16, 128, 16, 128, 16, 3, cache(**kw), None) == rc, kw
+        assert lib.vdit_kv_cache_read(cache(**kw), 16, 3, 16, 128, 16, 128, 0, None) == rc, kw
+    assert lib.vdit_kv_cache_write(16, 120, 16, 128, 16, 3, cache(), None) == -1
+    assert lib.vdit_kv_cache_write(16, 132, 16, 128, 16, 3, cache(), None) == -2
+    assert lib.vdit_kv_cache_write(16, 128, 16, 128, 16, 0, cache(), None) == 0
+    assert lib.vdit_kv_cache_write(16, 128, 16, 128, 16, 0, None, None) == -1
+    assert lib.vdit_kv_cache_read(cache(), 16, 3, 16, 128, 16, 128, 1, None) == -1
+    args = [16, 128, cache(), 16, 4, 4, 16, 1, 2, 0.125, 16, 128, None, 0, None]
+    need = lib.vdit_attention_1q_cached_workspace_bytes(1, 2, 2, 64, 512, 16)
     assert need > 0
-    for at, value, rc in ((16, 3, -1), (1, 120, -1), (12, -1, -1), (9, 80, -4), (10, 5, -4), (0, 8, -2), (15, 0, 0)):
+    for at, value, rc in ((8, 3, -1), (1, 120, -1), (4, -1, -1), (5, 1 << 30, -4), (2, cache(head_dim=80), -4),
+                          (2, None, -1), (0, 8, -2), (7, 0, 0)):
         a = list(args)
         a[at] = value
         assert lib.vdit_attention_1q_cached(*a) == rc, (at, value)
     a = list(args)
-    a[13], a[20], a[21] = 64, 16, need - 1
+    a[5], a[12], a[13] = 512, 16, need - 1
     assert lib.vdit_attention_1q_cached(*a) == -5
 
 
