@@ -74,6 +74,9 @@ SIGNATURES = {
     "vdit_mxfp4_quantize": (ctypes.c_int, [_vp, _c_i32, _c_i64, _c_i64, _c_i32, _vp, _vp, _vp]),
     "vdit_mxfp4_dequantize": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i32, _vp, _c_i32, _c_i64, _vp]),
     "vdit_linear_mxfp4": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp]),
+    "vdit_linear_mxfp4_dense_workspace_bytes": (_c_sz, [_c_i64, _c_i32]),
+    "vdit_linear_mxfp4_dense": (ctypes.c_int, [_vp, _c_i32, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32,
+                                               _vp, _c_sz, _vp]),
     "vdit_kv_cache_write": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp]),
     "vdit_kv_cache_read": (ctypes.c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i32, _vp]),
     "vdit_attention_1q_cached_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),

@@ -108,6 +108,14 @@ __device__ __forceinline__ uint2 encode8_e4m3(const float* f) {
     return r;
 }
 
+// the e2m1 value nearest to y, ties to even, no further than 6, in fp32: adding and taking away
+// 1.5 * 2^23 units rounds to a unit, half below 2, one below 4, two above.  (Where the codes are not
+// stored: encode8_e2m1 and decode8_e2m1 of its result in one kernel gave zeros, compiled by nvcc 12.9.)
+__device__ __forceinline__ float round_e2m1(float y) {
+    const float a = fabsf(y), big = a < 2.f ? 6291456.f : a < 4.f ? 12582912.f : 25165824.f;
+    return copysignf(fminf((a + big) - big, 6.f), y);
+}
+
 // codes to f16 pairs (every element value is an f16 value)
 __device__ __forceinline__ void decode8_e2m1(uint32_t c, __half2* h) {
     uint32_t r[4];

@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (every CTA)
         if (lane == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");          // a is written (when launched beside its writer)
             int it = 0;
             bool ok = true;
             for (int t = unit; ok && t < ntiles; t += nunits) {
@@ -365,6 +366,7 @@ struct Call {
     CUtensorMap out;
     Args p;
     int dev, sms;
+    bool after_quantize;
     cudaStream_t stream;
 };
 
@@ -373,10 +375,12 @@ int launch(const Call& c) {
     // units (CTAs or pairs) resident at once, asked once per device; 0: not asked yet
     static std::atomic<int> resident[kMaxDevices];
     const Args& p = c.p;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = CG;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = sizeof(Smem<CG, BN>) + 1024;
@@ -405,6 +409,7 @@ int launch(const Call& c) {
     const int64_t tiles = ((p.m + CG * BM - 1) / (CG * BM)) * ((p.n + BN - 1) / BN);
     if (tiles > INT32_MAX / 2) return VDIT_ERR_UNSUPPORTED;
     cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(tiles, units)));
+    cfg.numAttrs = c.after_quantize ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, linear_kernel<CG, BN>, ma, mw, msa, msw, c.out, p);
     if (e != cudaSuccess) {
         record_cuda_error(e);
@@ -452,9 +457,14 @@ int mxlinear_error_word(int clear) {
 using namespace vdit;
 using namespace vdit::mx;
 
-extern "C" int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
-                                 const void* bias, void* out, int64_t ldo, int64_t m, int32_t n, int32_t k,
-                                 vdit_stream_t stream) {
+namespace vdit {
+namespace mx {
+namespace {
+
+// The product of quantised rows; after_quantize: launched behind the kernel that writes a, beside whose
+// end it starts.
+int linear_codes(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales, const void* bias,
+                 void* out, int64_t ldo, int64_t m, int32_t n, int32_t k, bool after_quantize, cudaStream_t stream) {
     if (!a_codes || !a_scales || !w_codes || !w_scales || !out || m < 0 || n <= 0 || k <= 0 || ldo < n)
         return VDIT_ERR_ARG;
     if (n % 8 || k % kBlock || m > (int64_t)INT32_MAX - BM) return VDIT_ERR_UNSUPPORTED;
@@ -466,7 +476,7 @@ extern "C" int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, cons
     const int dev = current_device(&sms);
     if (dev < 0) return VDIT_ERR_UNSUPPORTED;
     Call c{a_codes, a_scales, w_codes, w_scales, {}, {static_cast<const __nv_bfloat16*>(bias), m, n, k}, dev, sms,
-           static_cast<cudaStream_t>(stream)};
+           after_quantize, stream};
     if (!make_map(&c.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, out, m, n, ldo * 2, 32, 64))
         return VDIT_ERR_DRIVER;
     switch (pick_tile(m, n, sms)) {
@@ -475,4 +485,212 @@ extern "C" int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, cons
         case 128: return launch<2, 128>(c);
         default: return launch<1, 64>(c);
     }
+}
+
+// ------------------------------------------------------------------ few dense rows
+// Up to 8 rows of a read the weight once and quantise themselves on the way: bound by latency for one
+// row, by the weight's bytes for wide ones.  A warp takes the four weight rows whose scales lie in one
+// vector (r, r + 32, r + 64, r + 96 of a 128-row block), a lane one block of 32 of each at a time; the
+// first blocks are on their way before the CTA quantises the rows of a into shared memory.  Products of
+// half a block are summed in f16 pairs, exactly: 8 products of at most 36, all multiples of 1/4, stay
+// below 2^11 quarters.  Across blocks the sums are fp32.
+constexpr int kFewRows = 8;
+constexpr int kFewWarps = 4;
+constexpr int64_t kFewElements = 65536;      // of a, rows rounded up: 136 KB of shared memory
+constexpr int kFewSmem = (int)(kFewElements * 2 + kFewElements / kBlock * 4);
+
+int few_rounded(int64_t m) { return m <= 2 ? (int)m : m <= 4 ? 4 : 8; }
+bool few_rows(int64_t m, int k) { return m <= kFewRows && (int64_t)few_rounded(m) * k <= kFewElements; }
+
+struct FewArgs {
+    const void* x;
+    int64_t ldx;
+    const uint8_t *w, *ws;
+    const __nv_bfloat16* bias;
+    __nv_bfloat16* out;
+    int64_t ldo;
+    int m, n, k;
+};
+
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 pair(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+
+// MT: rows of a, rounded up to a power of two (the rows past m are zeros)
+template <int T, int MT>
+__global__ void __launch_bounds__(kFewWarps * 32) few_rows_kernel(const __grid_constant__ FewArgs p) {
+    extern __shared__ __align__(16) uint8_t few[];
+    uint4* xs = reinterpret_cast<uint4*>(few);                          // [MT][blocks][4] chunks of 8 elements, f16
+    const int blocks = p.k / kBlock;
+    float* xscale = reinterpret_cast<float*>(few + (size_t)MT * p.k * 2);   // [MT][blocks]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int groups = scale_col_groups(p.k);
+    const int task = blockIdx.x * kFewWarps + warp;
+    const int row0 = (task >> 5) * 128 + (task & 31);
+    const bool live = row0 < p.n;
+    const uint8_t* scales = p.ws + (int64_t)(task >> 5) * groups * 512 + (task & 31) * 16;
+    uint4 c[4], s;
+    auto fetch = [&](int b) {                               // block b of the four rows
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            c[r] = live && b < blocks && row0 + 32 * r < p.n
+                       ? __ldg(reinterpret_cast<const uint4*>(p.w + (int64_t)(row0 + 32 * r) * (p.k / 2)) + b)
+                       : make_uint4(0, 0, 0, 0);
+        s = live && b < blocks ? __ldg(reinterpret_cast<const uint4*>(scales + (b >> 2) * 512)) : make_uint4(0, 0, 0, 0);
+    };
+    fetch(lane);
+
+    // quantise a: 8 elements a thread, four neighbouring threads a block; the 16-byte chunks of a
+    // block are rotated so that 8 lanes reading the same chunk of 8 blocks meet different banks
+    for (int i = threadIdx.x; i < MT * p.k / 8; i += kFewWarps * 32) {
+        const int row = i / (p.k / 8), at = i - row * (p.k / 8), b = at >> 2, j = at & 3;
+        float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (row < p.m) load8_f32(static_cast<const typename Elem<T>::type*>(p.x) + row * p.ldx + at * 8, f);
+        const unsigned quad = 0xfu << (threadIdx.x & 28);
+        uint32_t top = amax8(f);
+        top = max(top, __shfl_xor_sync(quad, top, 1));
+        top = max(top, __shfl_xor_sync(quad, top, 2));
+        const uint32_t e = scale_byte<4>(top);
+        const float inv = scale_inverse(e);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] = e == 255 ? 0.f : round_e2m1(f[q] * inv);
+        xs[(row * blocks + b) * 4 + (j ^ (b >> 1 & 3))] =
+            make_uint4(bits(__floats2half2_rn(f[0], f[1])), bits(__floats2half2_rn(f[2], f[3])),
+                       bits(__floats2half2_rn(f[4], f[5])), bits(__floats2half2_rn(f[6], f[7])));
+        if (j == 0) xscale[row * blocks + b] = scale_value(e);
+    }
+    __syncthreads();
+    if (!live) return;
+
+    float acc[4][MT];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[r][i] = 0.f;
+    for (int b0 = 0; b0 < blocks; b0 += 32) {
+        const int b = b0 + lane;
+        __half2 w[4][16];
+        float sc[4];
+        const uint32_t word[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            decode8_e2m1(c[r].x, w[r]);
+            decode8_e2m1(c[r].y, w[r] + 4);
+            decode8_e2m1(c[r].z, w[r] + 8);
+            decode8_e2m1(c[r].w, w[r] + 12);
+            sc[r] = scale_value((word[r] >> (8 * (b & 3))) & 255u);
+        }
+        if (b0 + 32 < blocks) fetch(b + 32);
+        if (b < blocks) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                __half2 x[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 u = xs[(i * blocks + b) * 4 + (j ^ (b >> 1 & 3))];
+                    x[4 * j] = pair(u.x);
+                    x[4 * j + 1] = pair(u.y);
+                    x[4 * j + 2] = pair(u.z);
+                    x[4 * j + 3] = pair(u.w);
+                }
+                const float e = xscale[i * blocks + b];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    __half2 h0 = __hmul2(w[r][0], x[0]), h1 = __hmul2(w[r][8], x[8]);
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) {
+                        h0 = __hfma2(w[r][j], x[j], h0);
+                        h1 = __hfma2(w[r][8 + j], x[8 + j], h1);
+                    }
+                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                    acc[r][i] = fmaf(((f0.x + f0.y) + (f1.x + f1.y)) * sc[r], e, acc[r][i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        if (i >= p.m) break;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float v = warp_sum(acc[r][i]);
+            const int col = row0 + 32 * r;
+            if (lane == r && col < p.n) p.out[i * p.ldo + col] = f2bf(v + (p.bias ? bf2f(p.bias[col]) : 0.f));
+        }
+    }
+}
+
+template <int T, int MT>
+int launch_few(const FewArgs& p, int dev, cudaStream_t s) {
+    static std::atomic<bool> ready[kMaxDevices];            // the largest shared memory size is set, per device
+    const size_t smem = (size_t)MT * p.k * 2 + (size_t)MT * (p.k / kBlock) * 4;
+    if (smem > 48 * 1024 && !ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   kFewSmem);
+        if (e != cudaSuccess) {
+            record_cuda_error(e);
+            return VDIT_ERR_LAUNCH;
+        }
+        ready[dev].store(true, std::memory_order_release);
+    }
+    const int tasks = (p.n + 127) / 128 * 32;
+    few_rows_kernel<T, MT><<<(tasks + kFewWarps - 1) / kFewWarps, kFewWarps * 32, smem, s>>>(p);
+    count_launches(1);
+    return check_launch();
+}
+
+template <int T>
+int launch_few(const FewArgs& p, int dev, cudaStream_t s) {
+    switch (few_rounded(p.m)) {
+        case 1: return launch_few<T, 1>(p, dev, s);
+        case 2: return launch_few<T, 2>(p, dev, s);
+        case 4: return launch_few<T, 4>(p, dev, s);
+        default: return launch_few<T, 8>(p, dev, s);
+    }
+}
+
+}  // namespace
+}  // namespace mx
+}  // namespace vdit
+
+extern "C" int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, const void* w_codes, const void* w_scales,
+                                 const void* bias, void* out, int64_t ldo, int64_t m, int32_t n, int32_t k,
+                                 vdit_stream_t stream) {
+    return linear_codes(a_codes, a_scales, w_codes, w_scales, bias, out, ldo, m, n, k, false,
+                        static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t vdit_linear_mxfp4_dense_workspace_bytes(int64_t m, int32_t k) {
+    if (m < 1 || k < 1 || few_rows(m, k)) return 0;
+    return (size_t)m * (k / 2) + vdit_mxfp4_scale_bytes(m, k);
+}
+
+extern "C" int vdit_linear_mxfp4_dense(const void* x, int32_t x_type, int64_t ldx, const void* w_codes,
+                                       const void* w_scales, const void* bias, void* out, int64_t ldo, int64_t m,
+                                       int32_t n, int32_t k, void* workspace, size_t workspace_bytes,
+                                       vdit_stream_t stream) {
+    const int elem = x_type == VDIT_F32 ? 4 : x_type == VDIT_BF16 || x_type == VDIT_F16 ? 2 : 0;
+    if (!elem || !x || !w_codes || !w_scales || !out || m < 0 || n <= 0 || k <= 0 || ldx < k || ldo < n)
+        return VDIT_ERR_ARG;
+    if (n % 8 || k % kBlock || m > (int64_t)INT32_MAX - BM) return VDIT_ERR_UNSUPPORTED;
+    if (!aligned16(x) || (ldx * elem) % 16 || !aligned16(w_codes) || !aligned16(w_scales) || !aligned16(out) ||
+        (bias && !aligned16(bias)) || ldo % 8)
+        return VDIT_ERR_ALIGN;
+    if (m == 0) return VDIT_OK;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (few_rows(m, k)) {
+        int sms;
+        const int dev = current_device(&sms);
+        if (dev < 0) return VDIT_ERR_UNSUPPORTED;
+        const FewArgs p{x, ldx, static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales),
+                        static_cast<const __nv_bfloat16*>(bias), static_cast<__nv_bfloat16*>(out), ldo, (int)m, n, k};
+        if (x_type == VDIT_BF16) return launch_few<VDIT_BF16>(p, dev, s);
+        if (x_type == VDIT_F16) return launch_few<VDIT_F16>(p, dev, s);
+        return launch_few<VDIT_F32>(p, dev, s);
+    }
+    if (!workspace || workspace_bytes < vdit_linear_mxfp4_dense_workspace_bytes(m, k)) return VDIT_ERR_WORKSPACE;
+    uint8_t* codes = static_cast<uint8_t*>(workspace);      // m * k / 2 bytes, a multiple of 16
+    uint8_t* scales = codes + m * (int64_t)(k / 2);
+    const int rc = vdit_mxfp4_quantize(x, x_type, ldx, m, k, codes, scales, stream);
+    if (rc != VDIT_OK) return rc;
+    return linear_codes(codes, scales, w_codes, w_scales, bias, out, ldo, m, n, k, true, s);
 }

@@ -30,6 +30,7 @@ template <int T>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const typename Elem<T>::type* __restrict__ x, int64_t ldx,
                                                             int64_t rows, int cols, int groups, int64_t units,
                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    asm volatile("griddepcontrol.launch_dependents;");      // a product of this matrix may set itself up meanwhile
     const int64_t u = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
     if (u >= units) return;                    // whole half warps leave; the shuffles below stay in one
     const int l = threadIdx.x & 15;

@@ -134,6 +134,11 @@ def dequantize_mxfp4(q: Mxfp4Tensor, dtype: torch.dtype = BF16) -> torch.Tensor:
     return out
 
 
+@lru_cache(maxsize=4096)
+def _dense_workspace(m: int, k: int) -> int:
+    return int(lib().vdit_linear_mxfp4_dense_workspace_bytes(m, k))
+
+
 def linear_mxfp4(a: Union[torch.Tensor, Mxfp4Tensor], w: Mxfp4Tensor, bias: Optional[torch.Tensor] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``linear`` on 4-bit operands: ``F.linear(a, w, bias)`` of the quantised values, fp32
@@ -143,7 +148,7 @@ def linear_mxfp4(a: Union[torch.Tensor, Mxfp4Tensor], w: Mxfp4Tensor, bias: Opti
     _check_mx("linear_mxfp4", "w", w)
     dense = torch.is_tensor(a)
     if dense:
-        _rows_view("linear_mxfp4", "a", a, _TYPES)
+        lda = _rows_view("linear_mxfp4", "a", a, _TYPES)
     else:
         _check_mx("linear_mxfp4", "a", a)
     m, k = a.shape
@@ -167,11 +172,16 @@ def linear_mxfp4(a: Union[torch.Tensor, Mxfp4Tensor], w: Mxfp4Tensor, bias: Opti
     if out is None:
         out = torch.empty((m, n), dtype=BF16, device=dev)
     if m:
+        pb = None if bias is None else bias.data_ptr()
         if dense:
-            a = quantize_mxfp4(a)
-        check(lib().vdit_linear_mxfp4(a.codes.data_ptr(), a.scales.data_ptr(), pw, w.scales.data_ptr(),
-                                      None if bias is None else bias.data_ptr(), out.data_ptr(), ldo, m, n, k,
-                                      _stream(dev.index)), "linear_mxfp4")
+            nb = _dense_workspace(m, k)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+            check(lib().vdit_linear_mxfp4_dense(a.data_ptr(), _TYPES[a.dtype], lda, pw, w.scales.data_ptr(), pb,
+                                                out.data_ptr(), ldo, m, n, k, None if ws is None else ws.data_ptr(), nb,
+                                                _stream(dev.index)), "linear_mxfp4")
+        else:
+            check(lib().vdit_linear_mxfp4(a.codes.data_ptr(), a.scales.data_ptr(), pw, w.scales.data_ptr(), pb,
+                                          out.data_ptr(), ldo, m, n, k, _stream(dev.index)), "linear_mxfp4")
     return out
 
 

@@ -95,6 +95,16 @@ def test_c_entry_points_check_before_any_launch():
     assert lib.vdit_linear_mxfp4(16, 16, 8, 16, None, 16, 64, 4, 64, 64, None) == -2
     assert lib.vdit_linear_mxfp4(16, 16, 16, 16, None, 16, 64, 0, 64, 64, None) == 0
 
+    assert lib.vdit_linear_mxfp4_dense_workspace_bytes(8, 1536) == 0
+    nb = lib.vdit_linear_mxfp4_dense_workspace_bytes(129, 160)
+    assert nb == 129 * 80 + 4 * 512
+    dense = [16, 0, 160, 16, 16, None, 16, 64, 129, 64, 160, 16, nb, None]
+    for at, value, rc in ((1, 5, -1), (2, 152, -1), (2, 164, -2), (9, 60, -4), (10, 144, -4), (7, 56, -1), (0, 8, -2),
+                          (11, None, -5), (12, nb - 1, -5), (8, 0, 0)):
+        a = list(dense)
+        a[at] = value
+        assert lib.vdit_linear_mxfp4_dense(*a) == rc, (at, value)
+
     def cache(**kw):
         a = dict(k=16, v=16, k_scales=16, v_scales=16, pages=2, page_size=16, heads=2, head_dim=64, bits=8)
         a.update(kw)
