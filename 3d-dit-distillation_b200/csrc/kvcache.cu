@@ -33,106 +33,149 @@ struct Cache {
     int page_size, page_shift, heads, hd;
 };
 
-// byte offsets of (slot, head)'s data and scales
-template <int BITS>
-__device__ __forceinline__ int64_t data_at(const Cache& c, int64_t page, int h, int off) {
-    return ((page * c.heads + h) * c.page_size + off) * (int64_t)(c.hd * BITS / 8);
-}
-__device__ __forceinline__ int64_t scale_at(const Cache& c, int64_t page, int h, int off) {
-    return ((page * c.heads + h) * c.page_size + off) * (int64_t)(c.hd / kBlock);
-}
-
 // ------------------------------------------------------------------ write and read back
-// Streams: a thread takes 8 channels of one row's key and value (four neighbouring threads one
-// block of 32), so a row's channels are read and its codes written by consecutive threads.
-template <int BITS>
-__device__ __forceinline__ void put8(const float* f, uint8_t* data, uint8_t* scale, bool first) {
-    uint32_t m = amax8(f);
-    const unsigned quad = 0xfu << (threadIdx.x & 28);
-    m = max(m, __shfl_xor_sync(quad, m, 1));
-    m = max(m, __shfl_xor_sync(quad, m, 2));
-    const uint32_t s = scale_byte<BITS>(m);
-    const float inv = scale_inverse(s);
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = s == 255 ? 0.f : f[j] * inv;
-    if (BITS == 4) *reinterpret_cast<uint32_t*>(data) = encode8_e2m1(y);
-    else *reinterpret_cast<uint2*>(data) = encode8_e4m3(y);
-    if (first) *scale = (uint8_t)s;
+// Streams: a thread takes half a block (16 channels) of the key and the value of kRowsAtOnce rows, all
+// its loads before the first store, so a row's channels are read and its codes written by consecutive
+// threads.  A CTA takes whole rows (as many as fit 256 threads, times kRowsAtOnce; a wider one in
+// steps), so that a thread's place takes no 64-bit division.
+constexpr int kRowsAtOnce = 2;
+struct Rows {
+    int64_t n;
+    int per_row, per_cta;                                   // half blocks of a row, rows of a CTA at once
+};
+
+// calls body(first row, rows apart, first channel) for the thread's half blocks; rows of n and more are
+// the body's to leave out
+template <typename F>
+__device__ __forceinline__ void each_half(const Rows& r, F&& body) {
+    const int mine = threadIdx.x / r.per_row;               // 0 when a row takes all threads
+    const int64_t row = (int64_t)blockIdx.x * r.per_cta * kRowsAtOnce + mine;
+    if (r.per_row > (int)blockDim.x) {
+        for (int i = threadIdx.x; i < r.per_row; i += blockDim.x) body(row, 1, i * 16);
+    } else if (mine < r.per_cta && row < r.n) {
+        body(row, r.per_cta, ((int)threadIdx.x - mine * r.per_row) * 16);
+    }
+}
+
+// a thread's place in the cache
+template <int HD, int BITS>
+__device__ __forceinline__ void place(const Cache& c, int64_t slot, int ch, int64_t* data, int64_t* scale) {
+    const int h = ch / HD, e = ch - h * HD;
+    const int64_t at = ((slot >> c.page_shift) * c.heads + h) * c.page_size + (slot & (c.page_size - 1));
+    *data = at * (HD * BITS / 8) + e * BITS / 8;
+    *scale = at * (HD / kBlock) + e / kBlock;
 }
 
 template <int BITS>
+__device__ __forceinline__ void put_half(const Half<VDIT_BF16>& x, uint8_t* data, uint8_t* scale) {
+    const unsigned pair = 3u << (threadIdx.x & 30);
+    uint32_t m = x.amax();
+    m = max(m, __shfl_xor_sync(pair, m, 1));
+    const uint32_t s = scale_byte<BITS>(m);
+    if (BITS == 4) *reinterpret_cast<uint2*>(data) = encode_half_e2m1(x, s);
+    else *reinterpret_cast<uint4*>(data) = encode_half_e4m3(x, s);
+    if (threadIdx.x % 2 == 0) *scale = (uint8_t)s;
+}
+
+template <int HD, int BITS>
 __global__ void __launch_bounds__(kThreads) write_kernel(const __nv_bfloat16* __restrict__ k, int64_t ldk,
                                                          const __nv_bfloat16* __restrict__ v, int64_t ldv,
-                                                         const int64_t* __restrict__ slots, int64_t n, Cache c) {
-    const int per_row = c.heads * c.hd / 8;
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t row = i / per_row;
-    if (row >= n) return;
-    const int ch = (int)(i - row * per_row) * 8;
-    const int64_t slot = __ldg(slots + row);
-    if (slot < 0) return;                                   // the four threads of a block agree
-    if (slot >= c.pages * c.page_size) {
-        atomicExch(&g_kvcache_error, kErrIndex);
-        return;
-    }
-    const int h = ch / c.hd, e = ch - h * c.hd;
-    const int64_t page = slot >> c.page_shift;
-    const int off = (int)(slot & (c.page_size - 1));
-    float fk[8], fv[8];
-    load8_f32(k + row * ldk + ch, fk);
-    load8_f32(v + row * ldv + ch, fv);
-    const int64_t d = data_at<BITS>(c, page, h, off) + e * BITS / 8, s = scale_at(c, page, h, off) + e / kBlock;
-    const bool first = (e & 31) == 0;
-    put8<BITS>(fk, c.k + d, c.ks + s, first);
-    put8<BITS>(fv, c.v + d, c.vs + s, first);
-}
-
-template <int BITS, typename T>
-__device__ __forceinline__ void get8(const uint8_t* data, const uint8_t* scale, T* out) {
-    const float s = scale_value(*scale);
-    __half2 h[4];
-    if (BITS == 4) {
-        decode8_e2m1(*reinterpret_cast<const uint32_t*>(data), h);
-    } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(data);
-        decode4_e4m3(u.x, h);
-        decode4_e4m3(u.y, h + 2);
-    }
-    float f[8];
+                                                         const int64_t* __restrict__ slots, Rows r, Cache c) {
+    each_half(r, [&](int64_t row0, int apart, int ch) {
+        int64_t slot[kRowsAtOnce];
+        Half<VDIT_BF16> a[kRowsAtOnce], b[kRowsAtOnce];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 t = __half22float2(h[j]);
-        f[2 * j] = t.x * s;
-        f[2 * j + 1] = t.y * s;
-    }
-    store8_f32(out, f);
+        for (int u = 0; u < kRowsAtOnce; ++u) {
+            const int64_t row = row0 + u * apart;
+            slot[u] = -1;
+            if (row < r.n) {
+                slot[u] = __ldg(slots + row);
+                a[u].load(k + row * ldk + ch);
+                b[u].load(v + row * ldv + ch);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRowsAtOnce; ++u) {
+            if (slot[u] < 0) continue;                      // both threads of a block agree
+            if (slot[u] >= c.pages * c.page_size) {
+                atomicExch(&g_kvcache_error, kErrIndex);
+                continue;
+            }
+            int64_t d, s;
+            place<HD, BITS>(c, slot[u], ch, &d, &s);
+            put_half<BITS>(a[u], c.k + d, c.ks + s);
+            put_half<BITS>(b[u], c.v + d, c.vs + s);
+        }
+    });
 }
 
-template <int BITS, typename T>
-__global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* __restrict__ slots, int64_t n,
+template <int BITS>
+struct HalfCodes {
+    uint4 u;
+    uint32_t s;
+    __device__ __forceinline__ void load(const uint8_t* data, const uint8_t* scale) {
+        if (BITS == 8) {
+            u = __ldg(reinterpret_cast<const uint4*>(data));
+        } else {
+            const uint2 t = __ldg(reinterpret_cast<const uint2*>(data));
+            u.x = t.x;
+            u.y = t.y;
+        }
+        s = __ldg(scale);
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T* out) const {
+        __half2 h[8];
+        if (BITS == 8) {
+            decode4_e4m3(u.x, h);
+            decode4_e4m3(u.y, h + 2);
+            decode4_e4m3(u.z, h + 4);
+            decode4_e4m3(u.w, h + 6);
+        } else {
+            decode8_e2m1(u.x, h);
+            decode8_e2m1(u.y, h + 4);
+        }
+        float f[16];
+        const float scale = scale_value(s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 t = fmul2(__half22float2(h[j]), scale);
+            f[2 * j] = t.x;
+            f[2 * j + 1] = t.y;
+        }
+        store_half(out, f);
+    }
+};
+
+template <int HD, int BITS, typename T>
+__global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* __restrict__ slots, Rows r,
                                                         T* __restrict__ k, int64_t ldk, T* __restrict__ v,
                                                         int64_t ldv) {
-    const int per_row = c.heads * c.hd / 8;
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t row = i / per_row;
-    if (row >= n) return;
-    const int ch = (int)(i - row * per_row) * 8;
-    const int64_t slot = __ldg(slots + row);
-    const bool outside = slot >= c.pages * c.page_size;
-    if (outside) atomicExch(&g_kvcache_error, kErrIndex);
-    if (slot < 0 || outside) {                              // no such row: zeros
-        const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        store8_f32(k + row * ldk + ch, z);
-        store8_f32(v + row * ldv + ch, z);
-        return;
-    }
-    const int h = ch / c.hd, e = ch - h * c.hd;
-    const int64_t page = slot >> c.page_shift;
-    const int off = (int)(slot & (c.page_size - 1));
-    const int64_t d = data_at<BITS>(c, page, h, off) + e * BITS / 8, s = scale_at(c, page, h, off) + e / kBlock;
-    get8<BITS>(c.k + d, c.ks + s, k + row * ldk + ch);
-    get8<BITS>(c.v + d, c.vs + s, v + row * ldv + ch);
+    each_half(r, [&](int64_t row0, int apart, int ch) {
+        int64_t slot[kRowsAtOnce];
+        HalfCodes<BITS> a[kRowsAtOnce], b[kRowsAtOnce];
+#pragma unroll
+        for (int u = 0; u < kRowsAtOnce; ++u) slot[u] = row0 + u * apart < r.n ? __ldg(slots + row0 + u * apart) : -1;
+#pragma unroll
+        for (int u = 0; u < kRowsAtOnce; ++u) {
+            a[u] = b[u] = HalfCodes<BITS>{make_uint4(0, 0, 0, 0), 0};
+            if (slot[u] >= c.pages * c.page_size) {
+                atomicExch(&g_kvcache_error, kErrIndex);
+            } else if (slot[u] >= 0) {                      // no such row: zeros
+                int64_t d, s;
+                place<HD, BITS>(c, slot[u], ch, &d, &s);
+                a[u].load(c.k + d, c.ks + s);
+                b[u].load(c.v + d, c.vs + s);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRowsAtOnce; ++u) {
+            const int64_t row = row0 + u * apart;
+            if (row >= r.n) continue;
+            a[u].store(k + row * ldk + ch);
+            b[u].store(v + row * ldv + ch);
+        }
+    });
 }
 
 // ------------------------------------------------------------------ single-query attention
@@ -698,11 +741,26 @@ int check_cache(const vdit_kv_cache* v, Cache* c) {
     return VDIT_OK;
 }
 
-// blocks of a launch over n rows of the cache's width, or 0 when they do not fit a grid
-int64_t row_blocks(const Cache& c, int64_t n) {
-    const int64_t per_row = (int64_t)c.heads * c.hd / 8;
-    const int64_t blocks = n > INT64_MAX / per_row - kThreads ? 0 : (n * per_row + kThreads - 1) / kThreads;
-    return blocks <= (int64_t)INT32_MAX ? blocks : 0;
+// a launch over n rows of the cache's width: CTAs and threads, 0 CTAs when they do not fit a grid
+Rows rows_of(const Cache& c, int64_t n, int64_t* ctas, int* threads) {
+    const int per_row = c.heads * c.hd / 16, per_cta = per_row < kThreads ? kThreads / per_row : 1;
+    *ctas = (n + (int64_t)per_cta * kRowsAtOnce - 1) / (per_cta * kRowsAtOnce);
+    if (*ctas > (int64_t)INT32_MAX) *ctas = 0;
+    *threads = per_row < kThreads ? (per_row * per_cta + 31) / 32 * 32 : kThreads;
+    return {n, per_row, per_cta};
+}
+
+// body(head_dim, bits) as constants
+template <typename F>
+void with_format(int hd, int bits, F&& body) {
+    auto sized = [&](auto b) {
+        if (hd == 32) body(std::integral_constant<int, 32>{}, b);
+        else if (hd == 64) body(std::integral_constant<int, 64>{}, b);
+        else if (hd == 96) body(std::integral_constant<int, 96>{}, b);
+        else body(std::integral_constant<int, 128>{}, b);
+    };
+    if (bits == 4) sized(std::integral_constant<int, 4>{});
+    else sized(std::integral_constant<int, 8>{});
 }
 
 }  // namespace
@@ -732,13 +790,15 @@ extern "C" int vdit_kv_cache_write(const void* k, int64_t ldk, const void* v, in
     if (!k || !v || !slots || n < 0 || ldk < d || ldv < d) return VDIT_ERR_ARG;
     if (!aligned16(k) || !aligned16(v) || ldk % 8 || ldv % 8) return VDIT_ERR_ALIGN;
     if (n == 0) return VDIT_OK;
-    const int64_t blocks = row_blocks(c, n);
-    if (!blocks) return VDIT_ERR_UNSUPPORTED;
+    int64_t ctas;
+    int threads;
+    const Rows r = rows_of(c, n, &ctas, &threads);
+    if (!ctas) return VDIT_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const auto* kp = static_cast<const __nv_bfloat16*>(k);
-    const auto* vp = static_cast<const __nv_bfloat16*>(v);
-    if (cache->bits == 4) write_kernel<4><<<(unsigned)blocks, kThreads, 0, s>>>(kp, ldk, vp, ldv, slots, n, c);
-    else write_kernel<8><<<(unsigned)blocks, kThreads, 0, s>>>(kp, ldk, vp, ldv, slots, n, c);
+    with_format(c.hd, cache->bits, [&](auto hd, auto bits) {
+        write_kernel<decltype(hd)::value, decltype(bits)::value><<<(unsigned)ctas, threads, 0, s>>>(
+            static_cast<const __nv_bfloat16*>(k), ldk, static_cast<const __nv_bfloat16*>(v), ldv, slots, r, c);
+    });
     count_launches(1);
     return check_launch();
 }
@@ -754,15 +814,20 @@ extern "C" int vdit_kv_cache_read(const vdit_kv_cache* cache, const int64_t* slo
     const int per16 = out_type == VDIT_F32 ? 4 : 8;
     if (!aligned16(k) || !aligned16(v) || ldk % per16 || ldv % per16) return VDIT_ERR_ALIGN;
     if (n == 0) return VDIT_OK;
-    const int64_t blocks = row_blocks(c, n);
-    if (!blocks) return VDIT_ERR_UNSUPPORTED;
+    int64_t ctas;
+    int threads;
+    const Rows r = rows_of(c, n, &ctas, &threads);
+    if (!ctas) return VDIT_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    auto run = [&](auto* kp, auto* vp) {
-        if (cache->bits == 4) read_kernel<4><<<(unsigned)blocks, kThreads, 0, s>>>(c, slots, n, kp, ldk, vp, ldv);
-        else read_kernel<8><<<(unsigned)blocks, kThreads, 0, s>>>(c, slots, n, kp, ldk, vp, ldv);
-    };
-    if (out_type == VDIT_F32) run(static_cast<float*>(k), static_cast<float*>(v));
-    else run(static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+    with_format(c.hd, cache->bits, [&](auto hd, auto bits) {
+        constexpr int HD = decltype(hd)::value, BITS = decltype(bits)::value;
+        if (out_type == VDIT_F32)
+            read_kernel<HD, BITS><<<(unsigned)ctas, threads, 0, s>>>(c, slots, r, static_cast<float*>(k), ldk,
+                                                                    static_cast<float*>(v), ldv);
+        else
+            read_kernel<HD, BITS><<<(unsigned)ctas, threads, 0, s>>>(c, slots, r, static_cast<__nv_bfloat16*>(k), ldk,
+                                                                    static_cast<__nv_bfloat16*>(v), ldv);
+    });
     count_launches(1);
     return check_launch();
 }
@@ -801,12 +866,9 @@ extern "C" int vdit_attention_1q_cached(const void* q, int64_t ldq, const vdit_k
                      ld_table, lengths, max_pages, heads, heads / kv_heads, plan.splits, plan.cluster,
                      softmax_scale * 1.4426950408889634f, static_cast<float*>(workspace)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    auto run = [&](auto hd) {
-        constexpr int HD = decltype(hd)::value;
-        return cache->bits == 4 ? launch_attend<HD, 4>(c, a, batch, s) : launch_attend<HD, 8>(c, a, batch, s);
-    };
-    if (head_dim == 32) return run(std::integral_constant<int, 32>{});
-    if (head_dim == 64) return run(std::integral_constant<int, 64>{});
-    if (head_dim == 96) return run(std::integral_constant<int, 96>{});
-    return run(std::integral_constant<int, 128>{});
+    int status = VDIT_OK;
+    with_format(c.hd, cache->bits, [&](auto hd, auto bits) {
+        status = launch_attend<decltype(hd)::value, decltype(bits)::value>(c, a, batch, s);
+    });
+    return status;
 }

@@ -2,11 +2,13 @@
 // block-scaled GEMM (mxlinear.cu).
 //
 // Both directions stream: rows x cols elements of 2 or 4 bytes on one side, 17 bytes per block of
-// 32 on the other, so HBM bounds them.  A half warp takes 128 columns (four blocks, 8 elements a
-// thread) of the four rows r, r + 32, r + 64, r + 96 of a 128-row block: its four 16-byte loads
-// are independent, and the four rows' scale words are the 16 consecutive bytes of one scale
-// block, so they leave (or arrive) as one vector.  The two half warps of a warp take
-// neighbouring r, which makes the scale vector a whole 32-byte sector.
+// 32 on the other, so HBM bounds them once the instructions an element takes are few: a thread takes
+// half a block at a time (16.7 instructions an element with a quarter block, 64-bit divisions for the
+// position and fp32 magnitudes: 42 us for 16384 x 3840 bf16, against 28 us).  Eight threads take
+// 128 columns (four blocks) of the four rows r, r + 32, r + 64, r + 96 of a 128-row block: their
+// loads are independent, and the four rows' scale words are the 16 consecutive bytes of one scale
+// block, so they leave (or arrive) as one vector.  A warp takes four neighbouring r, a CTA eight
+// groups of 128 columns of them.
 #include "mx.cuh"
 
 namespace vdit {
@@ -15,107 +17,89 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// unit (half warp) -> row block, first row in it, 128-column group
-struct Unit {
-    int64_t rb;
-    int r, g;
+// blockIdx.x: 128-row block and four rows r of its first 32; blockIdx.y and the warp: group of 128 columns
+struct Place {
+    int64_t row;      // r; the thread's rows are row + 32 i
+    int col;
+    int64_t scale;    // byte of the scale vector
 };
-__device__ __forceinline__ Unit unit_of(int64_t u, int groups) {
-    const int64_t pair = u >> 1;               // (row block, r / 2, group), group fastest
-    const int64_t rest = pair / groups;
-    return {rest >> 4, (int)(rest & 15) * 2 + (int)(u & 1), (int)(pair - rest * groups)};
+__device__ __forceinline__ Place place_of(int groups, int* group) {
+    const int g = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int64_t rb = blockIdx.x >> 3;
+    const int r = (blockIdx.x & 7) * 4 + (lane >> 3);
+    *group = g;
+    return {rb * 128 + r, g * 128 + (lane & 7) * 16, (rb * groups + g) * 512 + r * 16};
 }
 
 template <int T>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const typename Elem<T>::type* __restrict__ x, int64_t ldx,
-                                                            int64_t rows, int cols, int groups, int64_t units,
+                                                            int64_t rows, int cols, int groups,
                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     asm volatile("griddepcontrol.launch_dependents;");      // a product of this matrix may set itself up meanwhile
-    const int64_t u = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
-    if (u >= units) return;                    // whole half warps leave; the shuffles below stay in one
-    const int l = threadIdx.x & 15;
-    const unsigned half = 0xffffu << (threadIdx.x & 16);
-    const Unit un = unit_of(u, groups);
-    const int col = un.g * 128 + l * 8;
-    const bool in_cols = col < cols;           // cols is a multiple of 32: a block is in or out as one
-    float f[4][8];
+    int g;
+    const Place at = place_of(groups, &g);
+    if (g >= groups) return;                                // whole warps leave
+    const int part = threadIdx.x & 7;
+    const bool in_cols = at.col < cols;                     // cols is a multiple of 32: a block is in or out as one
+    Half<T> v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t row = un.rb * 128 + un.r + 32 * i;
-        if (in_cols && row < rows) {
-            load8_f32(x + row * ldx + col, f[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-        }
+        if (in_cols && at.row + 32 * i < rows) v[i].load(x + (at.row + 32 * i) * ldx + at.col);
+        else v[i].zero();
     }
     uint32_t word[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t row = un.rb * 128 + un.r + 32 * i;
-        uint32_t m = amax8(f[i]);
-        m = max(m, __shfl_xor_sync(half, m, 1));
-        m = max(m, __shfl_xor_sync(half, m, 2));
+        uint32_t m = v[i].amax();
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         const uint32_t s = scale_byte<4>(m);
-        const float inv = scale_inverse(s);
-        if (in_cols && row < rows) {
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = s == 255 ? 0.f : f[i][j] * inv;
-            *reinterpret_cast<uint32_t*>(codes + row * (cols / 2) + col / 2) = encode8_e2m1(y);
-        }
-        uint32_t w = s << (8 * (l >> 2));      // this block's byte of the row's scale word
-        w |= __shfl_xor_sync(half, w, 4);
-        w |= __shfl_xor_sync(half, w, 8);
-        word[i] = w;
+        if (in_cols && at.row + 32 * i < rows)
+            *reinterpret_cast<uint2*>(codes + (at.row + 32 * i) * (cols / 2) + at.col / 2) = encode_half_e2m1(v[i], s);
+        uint32_t w = s << (8 * (part >> 1));                // this block's byte of the row's scale word
+        w |= __shfl_xor_sync(0xffffffffu, w, 2);
+        word[i] = w | __shfl_xor_sync(0xffffffffu, w, 4);
     }
-    if (l == 0)
-        *reinterpret_cast<uint4*>(scales + (un.rb * groups + un.g) * 512 + un.r * 16) =
-            make_uint4(word[0], word[1], word[2], word[3]);
+    if (part == 0) *reinterpret_cast<uint4*>(scales + at.scale) = make_uint4(word[0], word[1], word[2], word[3]);
 }
 
 template <int T>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, int64_t rows,
-                                                              int cols, int groups, int64_t units,
+                                                              int cols, int groups,
                                                               typename Elem<T>::type* __restrict__ out, int64_t ldo) {
-    const int64_t u = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
-    if (u >= units) return;
-    const int l = threadIdx.x & 15;
-    const Unit un = unit_of(u, groups);
-    const int col = un.g * 128 + l * 8;
-    if (col >= cols) return;
-    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(scales + (un.rb * groups + un.g) * 512 + un.r * 16));
+    int g;
+    const Place at = place_of(groups, &g);
+    if (g >= groups || at.col >= cols) return;
+    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(scales + at.scale));
     const uint32_t word[4] = {sw.x, sw.y, sw.z, sw.w};
-    uint32_t c[4];
+    uint2 c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        c[i] = at.row + 32 * i < rows
+                   ? __ldg(reinterpret_cast<const uint2*>(codes + (at.row + 32 * i) * (cols / 2) + at.col / 2))
+                   : make_uint2(0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t row = un.rb * 128 + un.r + 32 * i;
-        c[i] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(codes + row * (cols / 2) + col / 2)) : 0u;
-    }
+        if (at.row + 32 * i >= rows) break;
+        const float s = scale_value((word[i] >> (8 * (threadIdx.x >> 1 & 3))) & 255u);
+        __half2 h[8];
+        decode8_e2m1(c[i].x, h);
+        decode8_e2m1(c[i].y, h + 4);
+        float f[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = un.rb * 128 + un.r + 32 * i;
-        if (row >= rows) break;
-        const float s = scale_value((word[i] >> (8 * (l >> 2))) & 255u);
-        __half2 h[4];
-        decode8_e2m1(c[i], h);
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 t = __half22float2(h[j]);
-            f[2 * j] = t.x * s;
-            f[2 * j + 1] = t.y * s;
+        for (int j = 0; j < 8; ++j) {
+            const float2 t = fmul2(__half22float2(h[j]), s);
+            f[2 * j] = t.x;
+            f[2 * j + 1] = t.y;
         }
-        store8_f32(out + row * ldo + col, f);
+        store_half(out + (at.row + 32 * i) * ldo + at.col, f);
     }
 }
 
-// blocks of a launch over rows x cols, or 0 when they do not fit a grid
-int64_t grid_of(int64_t rows, int cols, int64_t* units) {
-    *units = scale_row_blocks(rows) * 32 * scale_col_groups(cols);
-    const int64_t blocks = (*units * 16 + kThreads - 1) / kThreads;
-    return blocks <= (int64_t)INT32_MAX ? blocks : 0;
+// grid of a launch over rows x cols; x = 0 when it does not fit
+dim3 grid_of(int64_t rows, int cols) {
+    const int64_t x = scale_row_blocks(rows) * 8, y = (scale_col_groups(cols) + 7) / 8;
+    return x > (int64_t)INT32_MAX || y > 65535 ? dim3(0, 0) : dim3((unsigned)x, (unsigned)y);
 }
 
 // shape, stride and alignment checks shared by both directions (elem: bytes of a dense element)
@@ -147,16 +131,14 @@ extern "C" int vdit_mxfp4_quantize(const void* x, int32_t x_type, int64_t ldx, i
     if (!elem) return VDIT_ERR_ARG;
     const int rc = check_args(x, ldx, rows, cols, elem, codes, scales);
     if (rc != VDIT_OK || rows == 0) return rc;
-    int64_t units;
-    const int64_t blocks = grid_of(rows, cols, &units);
-    if (!blocks) return VDIT_ERR_UNSUPPORTED;
+    const dim3 grid = grid_of(rows, cols);
+    if (!grid.x) return VDIT_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int groups = scale_col_groups(cols);
     auto run = [&](auto tag) {
         constexpr int T = decltype(tag)::value;
-        quantize_kernel<T><<<(unsigned)blocks, kThreads, 0, s>>>(static_cast<const typename Elem<T>::type*>(x), ldx, rows,
-                                                                cols, groups, units, static_cast<uint8_t*>(codes),
-                                                                static_cast<uint8_t*>(scales));
+        quantize_kernel<T><<<grid, kThreads, 0, s>>>(static_cast<const typename Elem<T>::type*>(x), ldx, rows, cols, groups,
+                                                     static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
     };
     if (x_type == VDIT_BF16) run(std::integral_constant<int, VDIT_BF16>{});
     else if (x_type == VDIT_F16) run(std::integral_constant<int, VDIT_F16>{});
@@ -171,15 +153,14 @@ extern "C" int vdit_mxfp4_dequantize(const void* codes, const void* scales, int6
     if (!elem) return VDIT_ERR_ARG;
     const int rc = check_args(out, ldo, rows, cols, elem, codes, scales);
     if (rc != VDIT_OK || rows == 0) return rc;
-    int64_t units;
-    const int64_t blocks = grid_of(rows, cols, &units);
-    if (!blocks) return VDIT_ERR_UNSUPPORTED;
+    const dim3 grid = grid_of(rows, cols);
+    if (!grid.x) return VDIT_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int groups = scale_col_groups(cols);
     auto run = [&](auto tag) {
         constexpr int T = decltype(tag)::value;
-        dequantize_kernel<T><<<(unsigned)blocks, kThreads, 0, s>>>(
-            static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, cols, groups, units,
+        dequantize_kernel<T><<<grid, kThreads, 0, s>>>(
+            static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, cols, groups,
             static_cast<typename Elem<T>::type*>(out), ldo);
     };
     if (out_type == VDIT_BF16) run(std::integral_constant<int, VDIT_BF16>{});
