@@ -691,21 +691,26 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
         record_cuda_error(e);
         return VDIT_ERR_LAUNCH;
     }
+    const dim3 grid(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
-    cfg.blockDim = dim3(kWarps * 32);
-    cfg.dynamicSmemBytes = bytes;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attend_kernel<HD, BITS>, c, a);
-    if (e != cudaSuccess) {
-        record_cuda_error(e);
-        return VDIT_ERR_LAUNCH;
+    if (a.cluster > 1) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = a.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(kWarps * 32);
+        cfg.dynamicSmemBytes = bytes;
+        e = cudaLaunchKernelEx(&cfg, attend_kernel<HD, BITS>, c, a);
+        if (e != cudaSuccess) {
+            record_cuda_error(e);
+            return VDIT_ERR_LAUNCH;
+        }
+    } else {
+        attend_kernel<HD, BITS><<<grid, kWarps * 32, bytes, s>>>(c, a);
     }
     count_launches(1);
     if (a.splits > a.cluster) {

@@ -63,8 +63,9 @@ def _scale_bytes(rows: int, cols: int) -> int:
 
 class Mxfp4Tensor:
     """A quantised matrix [rows, cols]: ``codes`` uint8 [rows, cols / 2] (two elements a byte) and
-    ``scales`` uint8 in the block-scaled MMA's order (opaque to callers)."""
-    __slots__ = ("codes", "scales", "rows", "cols")
+    ``scales`` uint8 in the block-scaled MMA's order (opaque to callers).  ``quantize_mxfp4`` puts
+    both into one buffer and makes the two views when they are asked for."""
+    __slots__ = ("rows", "cols", "device", "_data", "_codes", "_scales", "_pc", "_ps")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         for t in (codes, scales):
@@ -75,21 +76,35 @@ class Mxfp4Tensor:
             raise ValueError(f"Mxfp4Tensor: {codes.numel()} codes and {scales.numel()} scale bytes are not those "
                              f"of [{rows}, {cols}]")
         _same_device("Mxfp4Tensor", codes, scales)
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        self.rows, self.cols, self.device = rows, cols, codes.device
+        self._data, self._codes, self._scales = None, codes, scales
+        self._pc, self._ps = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _of(cls, codes, scales, rows, cols) -> "Mxfp4Tensor":
+    def _new(cls, like: torch.Tensor, rows: int, cols: int) -> "Mxfp4Tensor":
         q = cls.__new__(cls)
-        q.codes, q.scales, q.rows, q.cols = codes, scales, rows, cols
+        at = rows * cols // 2                               # a multiple of 16
+        q._data = data = like.new_empty(at + _scale_bytes(rows, cols), dtype=torch.uint8)
+        q.rows, q.cols, q.device, q._codes, q._scales = rows, cols, data.device, None, None
+        q._pc = data.data_ptr()
+        q._ps = q._pc + at
         return q
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._data[:self.rows * self.cols // 2].view(self.rows, self.cols // 2)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._data[self.rows * self.cols // 2:]
+        return self._scales
 
     @property
     def shape(self) -> Tuple[int, int]:
         return (self.rows, self.cols)
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
 
 
 def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Tensor:
@@ -99,21 +114,25 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Tensor:
     m, k = x.shape
     if k == 0 or k % BLOCK:
         raise ValueError(f"quantize_mxfp4: {k} columns, not a multiple of {BLOCK}")
-    p, dev = ptr(x), x.device
+    p = ptr(x)
     if _elsewhere(x):
-        with torch.cuda.device(dev):
+        with torch.cuda.device(x.device):
             return quantize_mxfp4(x)
-    codes = torch.empty((m, k // 2), dtype=torch.uint8, device=dev)
-    scales = torch.empty(_scale_bytes(m, k), dtype=torch.uint8, device=dev)
+    q = Mxfp4Tensor._new(x, m, k)
     if m:
-        check(lib().vdit_mxfp4_quantize(p, _TYPES[x.dtype], ld, m, k, codes.data_ptr(), scales.data_ptr(),
-                                        _stream(dev.index)), "mxfp4_quantize")
-    return Mxfp4Tensor._of(codes, scales, m, k)
+        check(lib().vdit_mxfp4_quantize(p, _TYPES[x.dtype], ld, m, k, q._pc, q._ps, _stream(q.device.index)),
+              "mxfp4_quantize")
+    return q
 
 
 def _check_mx(what: str, name: str, q: Mxfp4Tensor) -> None:
     if not isinstance(q, Mxfp4Tensor):
         raise ValueError(f"{what}: {name} must be an Mxfp4Tensor, got {type(q).__name__}")
+
+
+def _need_cuda(dev: torch.device) -> None:
+    if dev.type != "cuda":
+        raise RuntimeError("vdit kernels need CUDA tensors (no CPU path)")
 
 
 def dequantize_mxfp4(q: Mxfp4Tensor, dtype: torch.dtype = BF16) -> torch.Tensor:
@@ -122,15 +141,15 @@ def dequantize_mxfp4(q: Mxfp4Tensor, dtype: torch.dtype = BF16) -> torch.Tensor:
     _check_mx("dequantize_mxfp4", "q", q)
     if dtype not in _TYPES:
         raise ValueError(f"dequantize_mxfp4: dtype must be bf16, fp16 or fp32, got {dtype}")
-    codes, m, k = q.codes, q.rows, q.cols
-    p, dev = ptr(codes), codes.device
-    if _elsewhere(codes):
+    m, k, dev = q.rows, q.cols, q.device
+    _need_cuda(dev)
+    if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return dequantize_mxfp4(q, dtype)
     out = torch.empty((m, k), dtype=dtype, device=dev)
     if m:
-        check(lib().vdit_mxfp4_dequantize(p, q.scales.data_ptr(), m, k, out.data_ptr(), _TYPES[dtype], k,
-                                          _stream(dev.index)), "mxfp4_dequantize")
+        check(lib().vdit_mxfp4_dequantize(q._pc, q._ps, m, k, out.data_ptr(), _TYPES[dtype], k, _stream(dev.index)),
+              "mxfp4_dequantize")
     return out
 
 
@@ -157,16 +176,18 @@ def linear_mxfp4(a: Union[torch.Tensor, Mxfp4Tensor], w: Mxfp4Tensor, bias: Opti
         raise ValueError(f"linear_mxfp4: a has {k} columns and w {w.cols}")
     if bias is not None and (bias.dtype != BF16 or bias.numel() != n or not bias.is_contiguous()):
         raise ValueError(f"linear_mxfp4: bias must be a contiguous bf16 vector of {n}")
-    wc = w.codes
     if out is None:
         ldo = n
     else:
         if out.dtype != BF16 or out.dim() != 2 or out.shape[0] < m or out.shape[1] < n:
             raise ValueError(f"linear_mxfp4: out must be a bf16 2D view of at least [{m}, {n}]")
         ldo = _rows_view("linear_mxfp4", "out", out, (BF16,))
-    _same_device("linear_mxfp4", wc, a if dense else a.codes, bias, out)
-    pw, dev = ptr(wc), wc.device
-    if _elsewhere(wc):
+    dev = w.device
+    for t in (a, bias, out):
+        if t is not None and t.device != dev:
+            raise ValueError(f"linear_mxfp4: tensors on {dev} and {t.device}")
+    _need_cuda(dev)
+    if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return linear_mxfp4(a, w, bias, out)
     if out is None:
@@ -176,12 +197,12 @@ def linear_mxfp4(a: Union[torch.Tensor, Mxfp4Tensor], w: Mxfp4Tensor, bias: Opti
         if dense:
             nb = _dense_workspace(m, k)
             ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-            check(lib().vdit_linear_mxfp4_dense(a.data_ptr(), _TYPES[a.dtype], lda, pw, w.scales.data_ptr(), pb,
-                                                out.data_ptr(), ldo, m, n, k, None if ws is None else ws.data_ptr(), nb,
+            check(lib().vdit_linear_mxfp4_dense(a.data_ptr(), _TYPES[a.dtype], lda, w._pc, w._ps, pb, out.data_ptr(),
+                                                ldo, m, n, k, None if ws is None else ws.data_ptr(), nb,
                                                 _stream(dev.index)), "linear_mxfp4")
         else:
-            check(lib().vdit_linear_mxfp4(a.codes.data_ptr(), a.scales.data_ptr(), pw, w.scales.data_ptr(), pb,
-                                          out.data_ptr(), ldo, m, n, k, _stream(dev.index)), "linear_mxfp4")
+            check(lib().vdit_linear_mxfp4(a._pc, a._ps, w._pc, w._ps, pb, out.data_ptr(), ldo, m, n, k,
+                                          _stream(dev.index)), "linear_mxfp4")
     return out
 
 
