@@ -420,7 +420,9 @@ int launch(const Call& c) {
 }
 
 // Tile for an [m, n] output: of the pairs' widths and the single CTA's 64 columns the one with
-// the least estimated time, rounds of tiles over the GPU x the time of a tile.
+// the least estimated time, rounds of tiles over the GPU x the time of a tile.  Measured at
+// k = 1536, us on 256 / 192 / 128 / 64 columns: 128 x 1536 7.9 / 6.9 / 6.7 / 5.5, 2048 x 1536
+// 8.7 / 8.2 / 9.6 / 10.0, 4101 x 1536 12.3 / 12.0 / 12.4 / 16.7, 4101 x 7680 27.9 / 31.7 / 38.0 / 60.2.
 int pick_tile(int64_t m, int n, int sms) {
     const int widths[4] = {256, 192, 128, 64};
     const double cost[4] = {1.0, 0.8, 0.6, 0.35};
@@ -488,18 +490,20 @@ int linear_codes(const void* a_codes, const void* a_scales, const void* w_codes,
 }
 
 // ------------------------------------------------------------------ few dense rows
-// Up to 8 rows of a read the weight once and quantise themselves on the way: bound by latency for one
-// row, by the weight's bytes for wide ones.  A warp takes the four weight rows whose scales lie in one
-// vector (r, r + 32, r + 64, r + 96 of a 128-row block), a lane one block of 32 of each at a time; the
-// first blocks are on their way before the CTA quantises the rows of a into shared memory.  Products of
-// half a block are summed in f16 pairs, exactly: 8 products of at most 36, all multiples of 1/4, stay
-// below 2^11 quarters.  Across blocks the sums are fp32.
-constexpr int kFewRows = 8;
-constexpr int kFewWarps = 4;
+// Up to 4 rows of a read the weight once and quantise themselves on the way, in one launch: bound by
+// latency.  A warp takes the four weight rows whose scales lie in one vector (r, r + 32, r + 64, r + 96
+// of a 128-row block), a lane one block of 32 of each at a time; the first blocks are on their way
+// before the CTA quantises the rows of a into shared memory.  Products of half a block are summed in
+// f16 pairs, exactly: 8 products of at most 36, all multiples of 1/4, stay below 2^11 quarters.  Across
+// blocks the sums are fp32.  Against quantising and the MMA kernel (for 7680 x 1536): one row 5.1
+// against 8.2 us, two 6.4; four 11.7, but with a launch less, which the host takes 5 us for; 8 rows
+// would take 18.5.
+constexpr int kFewRows = 4;
+constexpr int kFewWarps = 8;
 constexpr int64_t kFewElements = 65536;      // of a, rows rounded up: 136 KB of shared memory
 constexpr int kFewSmem = (int)(kFewElements * 2 + kFewElements / kBlock * 4);
 
-int few_rounded(int64_t m) { return m <= 2 ? (int)m : m <= 4 ? 4 : 8; }
+int few_rounded(int64_t m) { return m <= 2 ? (int)m : 4; }
 bool few_rows(int64_t m, int k) { return m <= kFewRows && (int64_t)few_rounded(m) * k <= kFewElements; }
 
 struct FewArgs {
@@ -539,24 +543,40 @@ __global__ void __launch_bounds__(kFewWarps * 32) few_rows_kernel(const __grid_c
     };
     fetch(lane);
 
-    // quantise a: 8 elements a thread, four neighbouring threads a block; the 16-byte chunks of a
-    // block are rotated so that 8 lanes reading the same chunk of 8 blocks meet different banks
-    for (int i = threadIdx.x; i < MT * p.k / 8; i += kFewWarps * 32) {
-        const int row = i / (p.k / 8), at = i - row * (p.k / 8), b = at >> 2, j = at & 3;
-        float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (row < p.m) load8_f32(static_cast<const typename Elem<T>::type*>(p.x) + row * p.ldx + at * 8, f);
-        const unsigned quad = 0xfu << (threadIdx.x & 28);
-        uint32_t top = amax8(f);
-        top = max(top, __shfl_xor_sync(quad, top, 1));
-        top = max(top, __shfl_xor_sync(quad, top, 2));
-        const uint32_t e = scale_byte<4>(top);
-        const float inv = scale_inverse(e);
+    // quantise a: half a block a thread, two of them at a time; the 16-byte chunks of a block are
+    // rotated so that 8 lanes reading the same chunk of 8 blocks meet different banks
+    const int per_row = p.k / 16, halves = MT * per_row;
+    for (int i0 = threadIdx.x; i0 < halves; i0 += 2 * kFewWarps * 32) {
+        Half<T> v[2];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) f[q] = e == 255 ? 0.f : round_e2m1(f[q] * inv);
-        xs[(row * blocks + b) * 4 + (j ^ (b >> 1 & 3))] =
-            make_uint4(bits(__floats2half2_rn(f[0], f[1])), bits(__floats2half2_rn(f[2], f[3])),
-                       bits(__floats2half2_rn(f[4], f[5])), bits(__floats2half2_rn(f[6], f[7])));
-        if (j == 0) xscale[row * blocks + b] = scale_value(e);
+        for (int u = 0; u < 2; ++u) {
+            const int i = i0 + u * kFewWarps * 32, row = i / per_row;
+            if (i < halves && row < p.m)
+                v[u].load(static_cast<const typename Elem<T>::type*>(p.x) + row * p.ldx + (i - row * per_row) * 16);
+            else
+                v[u].zero();
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = i0 + u * kFewWarps * 32;
+            if (i >= halves) break;                         // both threads of a block
+            const int at = i >> 1, j = (i & 1) * 2;         // block (of all rows) and first chunk
+            const unsigned two = 3u << (threadIdx.x & 30);
+            uint32_t top = v[u].amax();
+            top = max(top, __shfl_xor_sync(two, top, 1));
+            const uint32_t e = scale_byte<4>(top);
+            const float inv = scale_inverse(e);
+            uint32_t h[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float2 y = fmul2(v[u].pair(q), inv);
+                h[q] = e == 255 ? 0u : bits(__floats2half2_rn(round_e2m1(y.x), round_e2m1(y.y)));
+            }
+            const int turn = (at % blocks) >> 1 & 3;
+            xs[at * 4 + (j ^ turn)] = make_uint4(h[0], h[1], h[2], h[3]);
+            xs[at * 4 + ((j + 1) ^ turn)] = make_uint4(h[4], h[5], h[6], h[7]);
+            if (j == 0) xscale[at] = scale_value(e);
+        }
     }
     __syncthreads();
     if (!live) return;
@@ -643,8 +663,7 @@ int launch_few(const FewArgs& p, int dev, cudaStream_t s) {
     switch (few_rounded(p.m)) {
         case 1: return launch_few<T, 1>(p, dev, s);
         case 2: return launch_few<T, 2>(p, dev, s);
-        case 4: return launch_few<T, 4>(p, dev, s);
-        default: return launch_few<T, 8>(p, dev, s);
+        default: return launch_few<T, 4>(p, dev, s);
     }
 }
 

@@ -348,7 +348,7 @@ int vdit_linear_mxfp4(const void* a_codes, const void* a_scales, const void* w_c
 
 /* The same product with the rows of a given dense, x [m, ldx] of x_type (rows on 16-byte boundaries),
  * quantised in the call: into the workspace (vdit_linear_mxfp4_dense_workspace_bytes(m, k) bytes, 16-byte
- * aligned), or on the way for up to 8 rows (then 0 bytes). */
+ * aligned), or on the way for a few rows (then 0 bytes). */
 size_t vdit_linear_mxfp4_dense_workspace_bytes(int64_t m, int32_t k);
 int vdit_linear_mxfp4_dense(const void* x, int32_t x_type, int64_t ldx, const void* w_codes, const void* w_scales,
                             const void* bias, void* out, int64_t ldo, int64_t m, int32_t n, int32_t k,

@@ -121,7 +121,7 @@ def check_linear(got, x, w, bias):
 
 @pytest.mark.parametrize("m,n,k", [
     (1, 8, 32), (1, 1536, 1536), (1, 200, 3840), (2, 264, 96), (5, 1000, 160), (7, 64, 2080), (8, 136, 352),
-    (3, 48, 16384), (5, 24, 13088), (1, 16, 70016), (9, 136, 352), (16, 1536, 256), (17, 72, 64), (33, 200, 1280), (127, 128, 128), (128, 192, 256), (129, 200, 288),
+    (4, 136, 352), (3, 48, 16384), (5, 24, 13088), (1, 16, 70016), (9, 136, 352), (16, 1536, 256), (17, 72, 64), (33, 200, 1280), (127, 128, 128), (128, 192, 256), (129, 200, 288),
     (250, 1536, 1536), (300, 392, 1280), (1000, 776, 3840), (257, 7680, 160), (4101, 1536, 512), (20000, 384, 64)])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_linear_matches_64_bits(m, n, k, with_bias):

@@ -95,7 +95,7 @@ def test_c_entry_points_check_before_any_launch():
     assert lib.vdit_linear_mxfp4(16, 16, 8, 16, None, 16, 64, 4, 64, 64, None) == -2
     assert lib.vdit_linear_mxfp4(16, 16, 16, 16, None, 16, 64, 0, 64, 64, None) == 0
 
-    assert lib.vdit_linear_mxfp4_dense_workspace_bytes(8, 1536) == 0
+    assert lib.vdit_linear_mxfp4_dense_workspace_bytes(4, 1536) == 0
     nb = lib.vdit_linear_mxfp4_dense_workspace_bytes(129, 160)
     assert nb == 129 * 80 + 4 * 512
     dense = [16, 0, 160, 16, 16, None, 16, 64, 129, 64, 160, 16, nb, None]
