@@ -301,10 +301,20 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* s, int row) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(s) + (row * 3 >> 2);
     return __funnelshift_r(w[0], w[1], (row * 3 & 3) * 8);
 }
-// byte k of a word as 2^(byte - 127); 255 gives an infinity, which makes a NaN of the zeros that a
-// block with that scale holds
-__device__ __forceinline__ float word_scale(uint32_t w, int k) {
-    return __uint_as_float(max((k < 3 ? w >> (8 * k) & 255u : w >> 24) << 23, 0x00400000u));
+// the bytes of a word as 2^(byte - 127), two a conversion; 255 is a NaN
+template <int NB>
+__device__ __forceinline__ void word_scales(uint32_t w, float* s) {
+    uint32_t lo, hi;
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.bf16x2.ue8m0x2 %0, a;\n\t"
+        "cvt.rn.bf16x2.ue8m0x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+    s[0] = __uint_as_float(lo << 16);
+    if (NB > 1) s[1] = __uint_as_float(lo & 0xffff0000u);
+    if (NB > 2) s[2] = __uint_as_float(hi << 16);
+    if (NB > 3) s[3] = __uint_as_float(hi & 0xffff0000u);
 }
 
 // shared memory of a warp's ring and of the whole CTA
@@ -437,11 +447,12 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         }
         // S = K Q^T: this lane has keys g + 8r of queries 2t and 2t + 1
         float s[4][2];
-        uint32_t ksw[4], vsw[4];
+        float ksc[4][NB];
+        uint32_t vsw[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             s[r][0] = s[r][1] = 0.f;
-            ksw[r] = scale_word<NB>(st + R::KS, g + 8 * r);
+            word_scales<NB>(scale_word<NB>(st + R::KS, g + 8 * r), ksc[r]);
             vsw[r] = scale_word<NB>(st + R::VS, g + 8 * r);
         }
 #pragma unroll
@@ -456,7 +467,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
                 const uint32_t f0[4] = {ka[0], kb[0], ka[1], kb[1]}, f1[4] = {ka[2], kb[2], ka[3], kb[3]};
                 mma_f16(d, f0, q[k][0], q[k][1]);
                 mma_f16(d, f1, q[k][2], q[k][3]);
-                const float sa = word_scale(ksw[2 * h], k), sb = word_scale(ksw[2 * h + 1], k);
+                const float sa = ksc[2 * h][k], sb = ksc[2 * h + 1][k];
                 s[2 * h][0] = fmaf(d[0], sa, s[2 * h][0]);
                 s[2 * h][1] = fmaf(d[1], sa, s[2 * h][1]);
                 s[2 * h + 1][0] = fmaf(d[2], sb, s[2 * h + 1][0]);
@@ -512,6 +523,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             top[0] = __vmaxu2(top[0], __shfl_xor_sync(0xffffffffu, top[0], w));
             if (NB > 1) top[1] = __vmaxu2(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
         }
+        float vsc[4][NB];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) word_scales<NB>(vsw[r], vsc[r]);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
             // weights times 2^14 over the largest scale (2^127 at most), the product times its inverse
@@ -521,7 +535,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float fa = word_scale(vsw[2 * h], k) * inv, fb = word_scale(vsw[2 * h + 1], k) * inv;
+                const float fa = vsc[2 * h][k] * inv, fb = vsc[2 * h + 1][k] * inv;
                 const uint32_t b0 = transpose8(pack_f16(s[2 * h][0] * fa, s[2 * h][1] * fa));
                 const uint32_t b1 = transpose8(pack_f16(s[2 * h + 1][0] * fb, s[2 * h + 1][1] * fb));
                 uint32_t va[4], vb[4];                      // keys 2t, 2t + 1 and 2t + 8, 2t + 9 of the half
