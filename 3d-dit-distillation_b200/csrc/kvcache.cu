@@ -5,6 +5,7 @@
 // [pages, heads, page_size, head_dim * bits / 8] bytes and their scales
 // [pages, heads, page_size, head_dim / 32] bytes, so the keys of one head in one page are
 // consecutive: what one query head reads.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -426,6 +427,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i, i);
+    int seen = 0;                                           // whether any key of this warp counted
     int cur = 0, next = kStages - 1;                        // the stage of this step and the one its copies go to
     for (int i = 0; i < mine; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -436,6 +438,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         next = cur;
         cur = cur == kStages - 1 ? 0 : cur + 1;
         const bool whole = nl[0] + nl[1] == kGroup;
+        seen |= nl[0] + nl[1];
         if (!whole) {
             // keys that do not count: their values and scales, whatever is there, must not reach the sums
             for (int r = 0; r < kGroup; ++r) {
@@ -556,6 +559,12 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 
+    // a warp whose scores were all -inf (a query with infinities) has seen keys, unlike an empty one:
+    // alone it makes 0 / 0, not zeros
+    if (seen) {
+        m0 = fmaxf(m0, -FLT_MAX);
+        m1 = fmaxf(m1, -FLT_MAX);
+    }
     // join the warps through shared memory
 #pragma unroll
     for (int w = 4; w < 32; w <<= 1) {
@@ -594,7 +603,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         }
         const int h = kh * a.group + q0 + j;
         if (a.splits == 1) {
-            a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(ll == 0.f ? 0.f : acc / ll);
+            a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(mm == -INFINITY ? 0.f : acc / ll);
         } else if (a.cluster == 1) {
             float* x = a.ws + (((int64_t)b * a.heads + h) * a.splits + split) * (2 + HD);
             x[2 + e] = acc;
@@ -627,7 +636,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             acc = fmaf(load_cluster(so_at + i * 4, r), f, acc);
             ll = fmaf(load_cluster(joined_at + j * 8 + 4, r), f, ll);
         }
-        a.out[b * a.ldo + (int64_t)(kh * a.group + q0) * HD + i] = f2bf(ll == 0.f ? 0.f : acc / ll);
+        a.out[b * a.ldo + (int64_t)(kh * a.group + q0) * HD + i] = f2bf(mm == -INFINITY ? 0.f : acc / ll);
     }
     tc::cluster_sync();                                     // no CTA leaves while another reads its memory
 }
@@ -663,7 +672,7 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
     float acc = 0.f;
 #pragma unroll 8
     for (int i = 0; i < a.splits; ++i) acc = fmaf(base[i * (2 + HD) + 2 + e], weight[i], acc);
-    a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(ll == 0.f ? 0.f : acc / ll);
+    a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(mm == -INFINITY ? 0.f : acc / ll);
 }
 
 // How the keys of a sequence are split: two rounds of the CTAs that fit the GPU (3 of 4 warps on each
@@ -881,6 +890,7 @@ extern "C" int vdit_attention_1q_cached(const void* q, int64_t ldq, const vdit_k
     if (workspace_bytes < vdit_attention_1q_cached_workspace_bytes(batch, heads, kv_heads, head_dim, max_pages, page_size) ||
         (plan.splits > plan.cluster && !workspace))
         return VDIT_ERR_WORKSPACE;
+    if (workspace && !aligned16(workspace)) return VDIT_ERR_ALIGN;
     const AttnArgs a{static_cast<const __nv_bfloat16*>(q), ldq, static_cast<__nv_bfloat16*>(out), ldo, page_table,
                      ld_table, lengths, max_pages, heads, heads / kv_heads, plan.splits, plan.cluster,
                      softmax_scale * 1.4426950408889634f, static_cast<float*>(workspace)};

@@ -42,6 +42,7 @@ constexpr int EPI_WARPS = 8;             // two for each quarter of the 128 TMEM
 constexpr int kThreads = (2 + EPI_WARPS) * 32;
 constexpr int kErr = 0x4D58;            // "MX": a bounded wait of the linear ran out
 constexpr int kScaleBlock = 512;        // 128 rows x 4 scales
+constexpr int kMaxSize = INT32_MAX - 1024;   // tile coordinates stay int32
 
 template <int CG, int BN>
 struct __align__(1024) Smem {
@@ -469,7 +470,7 @@ int linear_codes(const void* a_codes, const void* a_scales, const void* w_codes,
                  void* out, int64_t ldo, int64_t m, int32_t n, int32_t k, bool after_quantize, cudaStream_t stream) {
     if (!a_codes || !a_scales || !w_codes || !w_scales || !out || m < 0 || n <= 0 || k <= 0 || ldo < n)
         return VDIT_ERR_ARG;
-    if (n % 8 || k % kBlock || m > (int64_t)INT32_MAX - BM) return VDIT_ERR_UNSUPPORTED;
+    if (n % 8 || k % kBlock || m > kMaxSize || n > kMaxSize || k > kMaxSize) return VDIT_ERR_UNSUPPORTED;
     if (!aligned16(a_codes) || !aligned16(a_scales) || !aligned16(w_codes) || !aligned16(w_scales) || !aligned16(out) ||
         (bias && !aligned16(bias)) || ldo % 8)
         return VDIT_ERR_ALIGN;
@@ -690,7 +691,7 @@ extern "C" int vdit_linear_mxfp4_dense(const void* x, int32_t x_type, int64_t ld
     const int elem = x_type == VDIT_F32 ? 4 : x_type == VDIT_BF16 || x_type == VDIT_F16 ? 2 : 0;
     if (!elem || !x || !w_codes || !w_scales || !out || m < 0 || n <= 0 || k <= 0 || ldx < k || ldo < n)
         return VDIT_ERR_ARG;
-    if (n % 8 || k % kBlock || m > (int64_t)INT32_MAX - BM) return VDIT_ERR_UNSUPPORTED;
+    if (n % 8 || k % kBlock || m > kMaxSize || n > kMaxSize || k > kMaxSize) return VDIT_ERR_UNSUPPORTED;
     if (!aligned16(x) || (ldx * elem) % 16 || !aligned16(w_codes) || !aligned16(w_scales) || !aligned16(out) ||
         (bias && !aligned16(bias)) || ldo % 8)
         return VDIT_ERR_ALIGN;

@@ -347,6 +347,39 @@ def test_attention_nan_stays_in_its_sequence_and_head():
     assert not bad[3].any()                                   # the NaN lies past this length
 
 
+def test_attention_with_infinities_in_queries():
+    """Scores of +-inf and NaN as a softmax has them: one at -inf weighs nothing, all at -inf or any
+    at +inf or NaN give NaN; other queries of the same key head are untouched."""
+    g = gen(8)
+    c = fk.MxKvCache(4, 16, 1, 32, bits=8, device=DEV)
+    k = torch.randn(64, 32, generator=g, device=DEV).to(BF16)
+    k[:, 0] = 1.0
+    k[5, 0] = -1.0
+    v = torch.randn(64, 32, generator=g, device=DEV).to(BF16)
+    fk.kv_cache_write(c, k, v, torch.arange(64, device=DEV))
+    q = torch.randn(4, 32, generator=g, device=DEV).to(BF16)
+    q[:3, 1:] = 0                                             # 0 * finite: the score is the first channel's
+    q[0, 0], q[1, 0], q[2, 0] = math.inf, -math.inf, math.nan
+    t = i32([[0, 1, 2, 3]])
+    got = fk.attention_1q_cached(q.reshape(1, 128), c, t, i32([64]))
+    o = host(got).reshape(4, 32)
+    assert np.isnan(o[:3]).all() and not np.isnan(o[3]).any()
+    # key 5 alone is at -inf for +inf and the other way round: 63 keys at +inf, then one at +inf
+    q2 = q.clone()
+    q2[0, 0], q2[1, 0] = -math.inf, -math.inf
+    k[:, 0] = 1.0
+    fk.kv_cache_write(c, k, v, torch.arange(64, device=DEV))  # every score -inf
+    o = host(fk.attention_1q_cached(q2.reshape(1, 128), c, t, i32([64]))).reshape(4, 32)
+    assert np.isnan(o[:3]).all() and not np.isnan(o[3]).any()
+    check_attend(got[:, 96:], q[3:], c, _first_key_negative(k), v, t, [64], 8)
+
+
+def _first_key_negative(k):
+    k = k.clone()
+    k[5, 0] = -1.0
+    return k
+
+
 def test_attention_one_table_for_all_and_bad_pages():
     g = gen(6)
     c, k, v = filled(g, 6, 32, 3, 96, 4)
@@ -362,6 +395,51 @@ def test_attention_one_table_for_all_and_bad_pages():
     check_attend(got[:2], q[:2], c, k, v, two, [64, 64], 4)
     check_attend(got[2:3], q[2:3], c, k, v, three, [96], 4)
     assert not got[3:].any()
+
+
+# ----------------------------------------------------------------------------- past 2^32
+
+def test_cache_past_four_gigabytes():
+    """Keys and values of 4.9 GB each: slots and pages at the end are where they should be."""
+    g = gen(13)
+    c = fk.MxKvCache(25000, 128, 12, 128, bits=8, device=DEV)
+    assert c.k.numel() > 2 ** 32
+    n = 300
+    slots = c.slots - 1 - torch.randperm(n, generator=g, device=DEV)
+    k, v = (torch.randn(n, c.width, generator=g, device=DEV).to(BF16) for _ in range(2))
+    fk.kv_cache_write(c, k, v, slots)
+    back = fk.kv_cache_read(c, slots)
+    assert same(host(back[0]), mxo.values(host(k), 8)) and same(host(back[1]), mxo.values(host(v), 8))
+    assert not c.k[:c.pages // 2].any() and not c.k[c.pages // 2:-3].any()
+    q = torch.randn(1, c.width, generator=g, device=DEV).to(BF16)
+    t = i32([[24998, 24999]])                                 # the last 256 slots, in order
+    tail = torch.arange(c.slots - 256, c.slots, device=DEV)
+    place = torch.empty(n, dtype=torch.int64, device=DEV)
+    place[c.slots - 1 - slots] = torch.arange(n, device=DEV)
+    rows_in = place[c.slots - 1 - tail]
+    small = fk.MxKvCache(2, 128, 12, 128, bits=8, device=DEV)
+    fk.kv_cache_write(small, k[rows_in], v[rows_in], torch.arange(256, device=DEV))
+    assert torch.equal(fk.attention_1q_cached(q, c, t, i32([256])),
+                       fk.attention_1q_cached(q, small, i32([[0, 1]]), i32([256])))
+
+
+def test_matrices_past_two_gigaelements():
+    g = gen(14)
+    m, k = 70000, 32768
+    x = torch.zeros(m, k, dtype=BF16, device=DEV)
+    tail = rows(g, 130, k)
+    x[-130:] = tail
+    q = fk.quantize_mxfp4(x)
+    del x
+    y = fk.dequantize_mxfp4(q)
+    assert same(host(y[-130:]), mxo.values(host(tail), 4)) and not y[:-130].any()
+    del y, q
+    m, n = 300000, 7680
+    x, w = rows(g, m, 32, spread=1.0), rows(g, n, 32, spread=1.0)
+    out = fk.linear_mxfp4(x, fk.quantize_mxfp4(w))
+    assert out.numel() > 2 ** 31
+    check_linear(out[-200:], x[-200:], w, None)
+    check_linear(out[:200], x[:200], w, None)
 
 
 # ----------------------------------------------------------------------------- together
@@ -434,8 +512,13 @@ def test_captured_and_on_another_stream():
     for seed in (21, 22, 23):
         fresh = [state(seed), state(seed + 100)]
         for s, f in zip(states, fresh):
-            for n in ("k", "v", "q", "slots"):
+            f["n"] = i32([60 - seed % 20, 7 * seed])           # past the last written slot: zeros
+            for n in ("k", "v", "q", "slots", "n"):
                 s[n].copy_(f[n])
+            s["c"].k.zero_()
+            s["c"].v.zero_()
+            s["c"].k_scales.zero_()
+            s["c"].v_scales.zero_()
         torch.cuda.synchronize()
         with torch.cuda.stream(side):
             want = [step(f) for f in fresh]
