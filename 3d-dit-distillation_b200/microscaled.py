@@ -16,27 +16,28 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from ._lib import KvCacheStruct, check, lib, ptr
+from ._lib import KvCacheStruct, check, lib
 
 BF16 = torch.bfloat16
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}     # VDIT_BF16, VDIT_F16, VDIT_F32
 BLOCK = 32                                                           # elements that share a scale
 
 # The calls here are a few microseconds of GPU work at their smallest, so the host path is kept
-# short: the raw stream handle, no device context unless another device is current, sizes kept.
+# short: raw stream handles and device indices, no device context unless another device is current.
 _stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
 
 
-def _elsewhere(t: torch.Tensor) -> bool:
-    """Whether the CUDA tensor is on another device than the current one."""
-    return t.get_device() != torch.cuda.current_device()
+def _need_cuda(index: int) -> None:
+    if index < 0:
+        raise RuntimeError("vdit kernels need CUDA tensors (no CPU path)")
 
 
-def _same_device(what: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
-    d = first.device
-    for t in rest:
-        if t is not None and t.device != d:
-            raise ValueError(f"{what}: tensors on {d} and {t.device}")
+def _same_device(what: str, index: int, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.get_device() != index:
+            raise ValueError(f"{what}: tensors on different devices ({t.device} and cuda:{index})" if index >= 0 else
+                             f"{what}: tensors on different devices ({t.device} and cpu)")
 
 
 def _rows_view(what: str, name: str, t: torch.Tensor, dtypes) -> int:
@@ -65,7 +66,7 @@ class Mxfp4Tensor:
     """A quantised matrix [rows, cols]: ``codes`` uint8 [rows, cols / 2] (two elements a byte) and
     ``scales`` uint8 in the block-scaled MMA's order (opaque to callers).  ``quantize_mxfp4`` puts
     both into one buffer and makes the two views when they are asked for."""
-    __slots__ = ("rows", "cols", "device", "_data", "_codes", "_scales", "_pc", "_ps")
+    __slots__ = ("rows", "cols", "_data", "_codes", "_scales", "_pc", "_ps", "_index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         for t in (codes, scales):
@@ -75,9 +76,9 @@ class Mxfp4Tensor:
                 scales.numel() != _scale_bytes(rows, cols)):
             raise ValueError(f"Mxfp4Tensor: {codes.numel()} codes and {scales.numel()} scale bytes are not those "
                              f"of [{rows}, {cols}]")
-        _same_device("Mxfp4Tensor", codes, scales)
-        self.rows, self.cols, self.device = rows, cols, codes.device
-        self._data, self._codes, self._scales = None, codes, scales
+        self._index = codes.get_device()
+        _same_device("Mxfp4Tensor", self._index, scales)
+        self.rows, self.cols, self._data, self._codes, self._scales = rows, cols, None, codes, scales
         self._pc, self._ps = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
@@ -85,10 +86,14 @@ class Mxfp4Tensor:
         q = cls.__new__(cls)
         at = rows * cols // 2                               # a multiple of 16
         q._data = data = like.new_empty(at + _scale_bytes(rows, cols), dtype=torch.uint8)
-        q.rows, q.cols, q.device, q._codes, q._scales = rows, cols, data.device, None, None
-        q._pc = data.data_ptr()
-        q._ps = q._pc + at
+        q.rows, q.cols, q._codes, q._scales, q._index = rows, cols, None, None, data.get_device()
+        q._pc = pc = data.data_ptr()
+        q._ps = pc + at
         return q
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
 
     @property
     def codes(self) -> torch.Tensor:
@@ -114,13 +119,14 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Tensor:
     m, k = x.shape
     if k == 0 or k % BLOCK:
         raise ValueError(f"quantize_mxfp4: {k} columns, not a multiple of {BLOCK}")
-    p = ptr(x)
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    index = x.get_device()
+    _need_cuda(index)
+    if index != _current():
+        with torch.cuda.device(index):
             return quantize_mxfp4(x)
     q = Mxfp4Tensor._new(x, m, k)
     if m:
-        check(lib().vdit_mxfp4_quantize(p, _TYPES[x.dtype], ld, m, k, q._pc, q._ps, _stream(q.device.index)),
+        check(lib().vdit_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], ld, m, k, q._pc, q._ps, _stream(index)),
               "mxfp4_quantize")
     return q
 
@@ -130,25 +136,20 @@ def _check_mx(what: str, name: str, q: Mxfp4Tensor) -> None:
         raise ValueError(f"{what}: {name} must be an Mxfp4Tensor, got {type(q).__name__}")
 
 
-def _need_cuda(dev: torch.device) -> None:
-    if dev.type != "cuda":
-        raise RuntimeError("vdit kernels need CUDA tensors (no CPU path)")
-
-
 def dequantize_mxfp4(q: Mxfp4Tensor, dtype: torch.dtype = BF16) -> torch.Tensor:
     """The values ``q`` stands for, [M, K] in ``dtype`` (exact in bf16 and fp32; fp16 rounds what
     lies outside its range)."""
     _check_mx("dequantize_mxfp4", "q", q)
     if dtype not in _TYPES:
         raise ValueError(f"dequantize_mxfp4: dtype must be bf16, fp16 or fp32, got {dtype}")
-    m, k, dev = q.rows, q.cols, q.device
-    _need_cuda(dev)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    m, k, index = q.rows, q.cols, q._index
+    _need_cuda(index)
+    if index != _current():
+        with torch.cuda.device(index):
             return dequantize_mxfp4(q, dtype)
-    out = torch.empty((m, k), dtype=dtype, device=dev)
+    out = (q._codes if q._data is None else q._data).new_empty((m, k), dtype=dtype)
     if m:
-        check(lib().vdit_mxfp4_dequantize(q._pc, q._ps, m, k, out.data_ptr(), _TYPES[dtype], k, _stream(dev.index)),
+        check(lib().vdit_mxfp4_dequantize(q._pc, q._ps, m, k, out.data_ptr(), _TYPES[dtype], k, _stream(index)),
               "mxfp4_dequantize")
     return out
 
@@ -182,27 +183,27 @@ def linear_mxfp4(a: Union[torch.Tensor, Mxfp4Tensor], w: Mxfp4Tensor, bias: Opti
         if out.dtype != BF16 or out.dim() != 2 or out.shape[0] < m or out.shape[1] < n:
             raise ValueError(f"linear_mxfp4: out must be a bf16 2D view of at least [{m}, {n}]")
         ldo = _rows_view("linear_mxfp4", "out", out, (BF16,))
-    dev = w.device
-    for t in (a, bias, out):
-        if t is not None and t.device != dev:
-            raise ValueError(f"linear_mxfp4: tensors on {dev} and {t.device}")
-    _need_cuda(dev)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    index = w._index
+    if (a.get_device() if dense else a._index) != index or (bias is not None and bias.get_device() != index) or \
+            (out is not None and out.get_device() != index):
+        raise ValueError("linear_mxfp4: tensors on different devices")
+    _need_cuda(index)
+    if index != _current():
+        with torch.cuda.device(index):
             return linear_mxfp4(a, w, bias, out)
     if out is None:
-        out = torch.empty((m, n), dtype=BF16, device=dev)
+        out = (a if dense else w._codes if w._data is None else w._data).new_empty((m, n), dtype=BF16)
     if m:
         pb = None if bias is None else bias.data_ptr()
         if dense:
             nb = _dense_workspace(m, k)
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+            ws = out.new_empty(nb, dtype=torch.uint8) if nb else None
             check(lib().vdit_linear_mxfp4_dense(a.data_ptr(), _TYPES[a.dtype], lda, w._pc, w._ps, pb, out.data_ptr(),
                                                 ldo, m, n, k, None if ws is None else ws.data_ptr(), nb,
-                                                _stream(dev.index)), "linear_mxfp4")
+                                                _stream(index)), "linear_mxfp4")
         else:
             check(lib().vdit_linear_mxfp4(a._pc, a._ps, w._pc, w._ps, pb, out.data_ptr(), ldo, m, n, k,
-                                          _stream(dev.index)), "linear_mxfp4")
+                                          _stream(index)), "linear_mxfp4")
     return out
 
 
@@ -230,6 +231,7 @@ class MxKvCache:
         self._k, self._v = (torch.zeros(*shape, head_dim * bits // 8, dtype=torch.uint8, device=device) for _ in range(2))
         self._ks, self._vs = (torch.zeros(*shape, head_dim // BLOCK, dtype=torch.uint8, device=device) for _ in range(2))
         self.device = self._k.device
+        self._index = self._k.get_device()
         self._struct = KvCacheStruct(*(t.data_ptr() for t in (self._k, self._v, self._ks, self._vs)), pages, page_size,
                                      kv_heads, head_dim, bits)
         self._ref = ctypes.addressof(self._struct)
@@ -257,15 +259,16 @@ def kv_cache_write(cache: MxKvCache, k: torch.Tensor, v: torch.Tensor, slots: to
     if k.shape != shape or v.shape != shape:
         raise ValueError(f"kv_cache_write: k and v must be [{n}, {cache.width}], got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
-    _same_device("kv_cache_write", cache._k, k, v, slots)
+    index = cache._index
+    _same_device("kv_cache_write", index, k, v, slots)
+    _need_cuda(index)
     if n == 0:
         return
-    pk = ptr(k)
-    if _elsewhere(k):
-        with torch.cuda.device(cache.device):
+    if index != _current():
+        with torch.cuda.device(index):
             return kv_cache_write(cache, k, v, slots)
-    check(lib().vdit_kv_cache_write(pk, ldk, v.data_ptr(), ldv, slots.data_ptr(), n, cache._ref,
-                                    _stream(cache.device.index)), "kv_cache_write")
+    check(lib().vdit_kv_cache_write(k.data_ptr(), ldk, v.data_ptr(), ldv, slots.data_ptr(), n, cache._ref,
+                                    _stream(index)), "kv_cache_write")
 
 
 def kv_cache_read(cache: MxKvCache, slots: torch.Tensor, dtype: torch.dtype = BF16) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -275,16 +278,17 @@ def kv_cache_read(cache: MxKvCache, slots: torch.Tensor, dtype: torch.dtype = BF
     n = _check_slots("kv_cache_read", cache, slots)
     if dtype is not BF16 and dtype is not torch.float32:
         raise ValueError(f"kv_cache_read: dtype must be bf16 or fp32, got {dtype}")
-    _same_device("kv_cache_read", cache._k, slots)
-    ps, dev, d = ptr(slots), cache.device, cache.width
-    if _elsewhere(slots):
-        with torch.cuda.device(dev):
+    index, d = cache._index, cache.width
+    _same_device("kv_cache_read", index, slots)
+    _need_cuda(index)
+    if index != _current():
+        with torch.cuda.device(index):
             return kv_cache_read(cache, slots, dtype)
-    k = torch.empty((n, d), dtype=dtype, device=dev)
-    v = torch.empty((n, d), dtype=dtype, device=dev)
+    k = slots.new_empty((n, d), dtype=dtype)
+    v = torch.empty_like(k)
     if n:
-        check(lib().vdit_kv_cache_read(cache._ref, ps, n, k.data_ptr(), d, v.data_ptr(), d,
-                                       _TYPES[dtype], _stream(dev.index)), "kv_cache_read")
+        check(lib().vdit_kv_cache_read(cache._ref, slots.data_ptr(), n, k.data_ptr(), d, v.data_ptr(), d,
+                                       _TYPES[dtype], _stream(index)), "kv_cache_read")
     return k, v
 
 
@@ -313,20 +317,21 @@ def attention_1q_cached(q: torch.Tensor, cache: MxKvCache, page_table: torch.Ten
                          f"got {tuple(page_table.shape)} {page_table.dtype}")
     if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != b or not lengths.is_contiguous():
         raise ValueError(f"{what}: lengths must be a contiguous int32 [{b}], got {tuple(lengths.shape)} {lengths.dtype}")
-    _same_device(what, cache._k, q, page_table, lengths)
-    pq, dev = ptr(q), cache.device
-    if _elsewhere(q):
-        with torch.cuda.device(dev):
+    index = cache._index
+    _same_device(what, index, q, page_table, lengths)
+    _need_cuda(index)
+    if index != _current():
+        with torch.cuda.device(index):
             return attention_1q_cached(q, cache, page_table, lengths, scale)
-    out = torch.empty((b, d), dtype=BF16, device=dev)
+    out = q.new_empty((b, d))
     if b:
         hd, pages = cache.head_dim, page_table.shape[1]
         heads = d // hd
         nb = _attend_workspace(b, heads, cache.kv_heads, hd, pages, cache.page_size)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        check(lib().vdit_attention_1q_cached(pq, ldq, cache._ref, page_table.data_ptr(),
+        ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
+        check(lib().vdit_attention_1q_cached(q.data_ptr(), ldq, cache._ref, page_table.data_ptr(),
                                              page_table.stride(0) if b > 1 else pages, pages, lengths.data_ptr(), b,
                                              heads, 1.0 / math.sqrt(hd) if scale is None else float(scale),
                                              out.data_ptr(), d, None if ws is None else ws.data_ptr(), nb,
-                                             _stream(dev.index)), what)
+                                             _stream(index)), what)
     return out
