@@ -24,36 +24,6 @@ template <> struct Elem<VDIT_BF16> { using type = __nv_bfloat16; };
 template <> struct Elem<VDIT_F16> { using type = __half; };
 template <> struct Elem<VDIT_F32> { using type = float; };
 
-// 8 consecutive elements as fp32 (16-byte loads)
-__device__ __forceinline__ void load8_f32(const __nv_bfloat16* p, float* f) { load8_nc(p, f); }
-__device__ __forceinline__ void load8_f32(const __half* p, float* f) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 t = __half22float2(h[i]);
-        f[2 * i] = t.x;
-        f[2 * i + 1] = t.y;
-    }
-}
-__device__ __forceinline__ void load8_f32(const float* p, float* f) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-__device__ __forceinline__ void store8_f32(__nv_bfloat16* p, const float* f) { store8(p, f); }
-__device__ __forceinline__ void store8_f32(__half* p, const float* f) {
-    uint4 u;
-    __half2* h = reinterpret_cast<__half2*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = u;
-}
-__device__ __forceinline__ void store8_f32(float* p, const float* f) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
-
 __device__ __forceinline__ float2 fmul2(float2 a, float s) {
     unsigned long long ra, rs, rd;
     asm("mov.b64 %0, {%1,%2};" : "=l"(ra) : "f"(a.x), "f"(a.y));

@@ -262,7 +262,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
             for (int c = lane * 8; c < BN; c += 256) {      // n is a multiple of 8
                 float bv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
                 if (p.bias && col0 + c < p.n) load8_nc(p.bias + col0 + c, bv);
-                store8_f32(bias + c, bv);
+                *reinterpret_cast<float4*>(bias + c) = make_float4(bv[0], bv[1], bv[2], bv[3]);
+                *reinterpret_cast<float4*>(bias + c + 4) = make_float4(bv[4], bv[5], bv[6], bv[7]);
             }
             __syncwarp();
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.acc_full[buf]), (lt >> 1) & 1, abort_flag,
