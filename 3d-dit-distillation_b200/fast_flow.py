@@ -23,7 +23,7 @@ import math
 from collections import OrderedDict
 from dataclasses import dataclass
 from pathlib import Path
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, List, Optional, Sequence
 
 import torch
 
@@ -41,9 +41,14 @@ KERNEL_CLASSES = {
     "attention_window_self": "tensor", "attention_voxel_to_context": "tensor",
     "attention_context_to_voxel": "tensor", "attention_context_self": "tensor",
     "gemm_qkv_fused": "tensor", "gemm_voxel": "tensor", "gemm_context": "tensor",
-    "dwconv27_swiglu": "hbm", "gate_add_modulate": "hbm", "single_query_context_to_voxel": "hbm",
+    "gemm_voxel_mxfp4": "tensor", "dwconv27_swiglu": "hbm", "gate_add_modulate": "hbm", "single_query_context_to_voxel": "hbm",
     "unpatchify_project": "hbm",
 }
+
+# The voxel-side linears that can run on 4-bit operands (``mxfp4_linears``): most of a block's FLOPs.
+# to_qkv stays in bf16 (its GEMM carries the QK norm, RoPE and window order), the context side too
+# (4101 rows, and its vector in the 1-token branch reads the weights in bf16).
+MXFP4_LINEARS = ("to_out", "to_qkv_cross", "to_q_cross", "to_out_cross", "ffn0", "ffn1")
 
 
 def _time_encoding(t: torch.Tensor, dim: int, max_period: float = 10000.0) -> torch.Tensor:
@@ -80,7 +85,11 @@ class OptimizedLatDitRunner:
     """Runs ``FlowModel`` NFEs and the exact sampler on one CUDA device."""
 
     def __init__(self, model, solver_config: Optional[SolverConfig] = None, weights_dir: Optional[Path] = None,
-                 device: Optional[torch.device] = None, cuda_graph: bool = False):
+                 device: Optional[torch.device] = None, cuda_graph: bool = False,
+                 mxfp4_linears: Sequence[str] = ()):
+        unknown = sorted(set(mxfp4_linears) - set(MXFP4_LINEARS))
+        if unknown:
+            raise ValueError(f"mxfp4_linears: {unknown} are not among {MXFP4_LINEARS}")
         if hasattr(model, "core") and not isinstance(model, LatDitModel):   # a reference LatDitModel
             core = model.core
             mc = dict(core.model_config, latent_scale=float(core.latent_scale))
@@ -122,6 +131,10 @@ class OptimizedLatDitRunner:
         self._wide_1q = self.num_heads <= 16 and self.dim % 128 == 0 and self.dim <= 2048 and self.head_dim <= 256
         # CUDA-graph replay of the sampler (per voxel count, context length and schedule)
         self.cuda_graph = bool(cuda_graph)
+        # block linears held and multiplied in 4-bit microscaled form (approximate; off by default)
+        self.mxfp4_linears = tuple(mxfp4_linears)
+        if self.mxfp4_linears and (a.dim % 32 or a.ffn_dim % 32):
+            raise ValueError(f"mxfp4_linears: widths {a.dim} and {a.ffn_dim} must be multiples of 32")
         self._graphs: "OrderedDict[tuple, _SampleGraph]" = OrderedDict()
         self.max_graphs = 4
         self._prepare_weights_and_buffers()
@@ -202,6 +215,9 @@ class OptimizedLatDitRunner:
                 bv = f32(p + "cond_to_kv_cross.bias")[D:]
                 Wox, box = f32(p + "to_out_cross.weight"), f32(p + "to_out_cross.bias")
                 w["cr1_w"], w["cr1_b"] = (Wox @ Wv).to(BF16), (Wox @ bv + box).to(BF16)
+            for n in self.mxfp4_linears:
+                if n in w:
+                    w[n] = fk.quantize_mxfp4(w[n])
             self.blocks.append(w)
         if a.depth > cd:
             # the constant cross-attention maps of the plain blocks, one batched GEMV per NFE
@@ -232,8 +248,11 @@ class OptimizedLatDitRunner:
         kt.setdefault(kind, []).append((e0, e1, float(units), self._nfe_shared))
         return out
 
-    def _lin(self, a: torch.Tensor, w: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
-        """A block linear on the tcgen05 GEMM (voxel rows or context rows)."""
+    def _lin(self, a: torch.Tensor, w, b: torch.Tensor) -> torch.Tensor:
+        """A block linear on the tcgen05 GEMM (voxel rows or context rows; a weight in 4 bits on the
+        block-scaled one)."""
+        if isinstance(w, fk.Mxfp4Tensor):
+            return self._run("gemm_voxel_mxfp4", 2.0 * a.shape[0] * a.shape[1] * w.rows, fk.linear_mxfp4, a, w, b)
         kind = "gemm_context" if a.shape[0] == self._ctx_rows else "gemm_voxel"
         return self._run(kind, 2.0 * a.shape[0] * a.shape[1] * w.shape[0], fk.linear, a, w, b)
 

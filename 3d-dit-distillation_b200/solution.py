@@ -116,14 +116,15 @@ class Solution(LatDitGenerator):
 
     def __init__(self, inner: LatDitModel, solver_config: Optional[SolverConfig] = None,
                  weights_dir: Optional[Path] = None, device: Optional[torch.device] = None,
-                 cuda_graph: bool = False):
+                 cuda_graph: bool = False, mxfp4_linears: Sequence[str] = ()):
         self.inner = inner
         self.solver_config = solver_config or SolverConfig()
         sc = self.solver_config
         self._default_runtime = FlowMatchSamplingParams(guidance_scale=sc.guidance_scale, cfg_range=sc.cfg_range,
                                                         rescale_t=sc.rescale_t,
                                                         num_inference_steps=sc.num_inference_steps)
-        self.runner = OptimizedLatDitRunner(inner, sc, weights_dir=weights_dir, device=device, cuda_graph=cuda_graph)
+        self.runner = OptimizedLatDitRunner(inner, sc, weights_dir=weights_dir, device=device, cuda_graph=cuda_graph,
+                                            mxfp4_linears=mxfp4_linears)
 
     @classmethod
     def from_pretrained(cls, pretrained_model_name_or_path: Union[str, os.PathLike],
@@ -144,7 +145,7 @@ class Solution(LatDitGenerator):
         if device is not None:
             device = torch.device(f"cuda:{device}" if isinstance(device, int) else device)
         inst = cls(model, solver_config=solver, weights_dir=primary, device=device,
-                   cuda_graph=bool(kwargs.get("cuda_graph", False)))
+                   cuda_graph=bool(kwargs.get("cuda_graph", False)), mxfp4_linears=kwargs.get("mxfp4_linears", ()))
         if solver.warmup_on_load:
             inst.runner.warmup()
         return inst
@@ -156,7 +157,8 @@ class Solution(LatDitGenerator):
         dev = kwargs.get("device", args[0] if args else None)
         if dev is not None:
             self.runner = OptimizedLatDitRunner(self.inner, self.solver_config, self.runner.weights_dir,
-                                                device=torch.device(dev), cuda_graph=self.runner.cuda_graph)
+                                                device=torch.device(dev), cuda_graph=self.runner.cuda_graph,
+                                                mxfp4_linears=self.runner.mxfp4_linears)
         return self
 
     def eval(self) -> "Solution":

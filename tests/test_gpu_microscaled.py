@@ -527,3 +527,66 @@ def test_captured_and_on_another_stream():
         torch.cuda.synchronize()
         for (_, got), w in zip(graphs, want):
             assert all(torch.equal(a, b) for a, b in zip(got, w))
+
+
+# ----------------------------------------------------------------------------- on the model's path
+
+def _model(dim=256, depth=3, cond_depth=2, n=700, side=8):
+    from oracle import model as om
+    from tests.golden.make_golden import shell_voxels
+    from vdit.model import LatDitModel
+    cfg = om.ModelConfig(dim=dim, head_dim=128, depth=depth, cond_depth=cond_depth, res=64, patch_size=256)
+    p = om.init_params(cfg, 5, weight_std=0.03, bias_std=0.02, scale_jitter=0.1)
+    mc = {"dim": dim, "head_dim": 128, "depth": depth, "cond_depth": cond_depth, "res": 64, "patch_size": 256,
+          "latent_scale": cfg.latent_scale}
+    gg = torch.Generator().manual_seed(6)
+    vox = shell_voxels(n, 64, 22.0, 6)
+    return (LatDitModel.from_state_dict(p, mc), torch.from_numpy(vox).to(DEV),
+            torch.randn(5 + side * side, dim, generator=gg).to(DEV, BF16), torch.randn(n, 16, generator=gg).to(DEV))
+
+
+def test_runner_runs_the_named_linears_in_four_bits(monkeypatch):
+    """Every voxel-side linear that is named goes through linear_mxfp4 on its own weight, in both
+    branches, and no other; each result is the one of that call's operands."""
+    from vdit.fast_flow import MXFP4_LINEARS, OptimizedLatDitRunner
+    from vdit.fast_sampler import SolverConfig
+    model, vox, ctx, xt = _model()
+    r = OptimizedLatDitRunner(model, SolverConfig(), device=torch.device(DEV), mxfp4_linears=MXFP4_LINEARS)
+    of = {id(w[n]): (b, n) for b, w in enumerate(r.blocks) for n in MXFP4_LINEARS if n in w}
+    assert len(of) == 3 * 4 + 2 + 1                           # two context blocks, one plain block
+    for (b, n), q in ((of[id(w[n])], w[n]) for w in r.blocks for n in MXFP4_LINEARS if n in w):
+        want = model.state[f"flow.blocks.{b}.{n}.weight"].to(BF16)
+        if n == "ffn0" and r.ffn_interleaved:
+            want = want[r.ffn_perm.cpu()]
+        assert same(host(fk.dequantize_mxfp4(q)), mxo.values(host(want), 4))
+    calls, real = [], fk.linear_mxfp4
+
+    def record(a, w, bias=None, out=None):
+        got = real(a, w, bias, out)
+        calls.append((of[id(w)], a.clone(), w, bias, got.clone()))
+        return got
+
+    monkeypatch.setattr(fk, "linear_mxfp4", record)
+    geom = r._prepare_sample_geometry([vox], ctx)
+    pos = r.forward_flow_fast(xt, 0.75, ctx, None, geom)
+    names = sorted(c[0] for c in calls)
+    assert names == sorted(of.values())
+    neg = r.forward_flow_fast(xt, 0.75, None, None, geom, uncond=True)
+    assert torch.isfinite(pos).all() and torch.isfinite(neg).all()
+    # the 1-token branch has constant cross-attention outputs, and shares block 0's self-attention
+    assert sorted(c[0] for c in calls[len(names):]) == sorted(
+        [(b, n) for b in range(3) for n in ("ffn0", "ffn1")] + [(b, "to_out") for b in (1, 2)])
+    torch.cuda.synchronize()
+    for (b, n), a, w, bias, got in calls[::4]:
+        check_linear(got, a, fk.dequantize_mxfp4(w), bias)
+
+
+def test_runner_in_four_bits_captured():
+    from vdit.fast_flow import OptimizedLatDitRunner
+    from vdit.fast_sampler import SolverConfig
+    model, vox, ctx, xt = _model()
+    r = OptimizedLatDitRunner(model, SolverConfig(), device=torch.device(DEV), mxfp4_linears=("ffn0", "ffn1"))
+    eager = r.sample_with_context(vox, ctx, noise=xt)
+    graphed = [r.sample_with_context(vox, ctx, noise=xt, cuda_graph=True) for _ in range(2)]
+    assert torch.isfinite(eager).all()
+    assert torch.equal(graphed[0], graphed[1]) and torch.equal(graphed[0], eager)

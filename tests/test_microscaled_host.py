@@ -145,3 +145,9 @@ def test_cache_addresses_stay_inside_and_apart(pages, page, heads, hd, bits):
         p, h, o = np.meshgrid(np.arange(pages), np.arange(heads), np.arange(page), indexing="ij")
         at = ((p * heads + h) * page + o) * width
         assert len(np.unique(at)) == at.size and at.max() + width == nb
+
+
+def test_runner_refuses_unknown_four_bit_linears():
+    from vdit.fast_flow import OptimizedLatDitRunner
+    with pytest.raises(ValueError, match="to_qkv"):
+        OptimizedLatDitRunner(None, mxfp4_linears=("ffn0", "to_qkv"))
