@@ -195,12 +195,14 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 //   S = K Q^T   32 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
 //               query by a power of two that puts its largest channel at 2^13: exact but for
 //               channels 2^27 below that one
-//   O += V^T P  channels x queries, P = 2^(s - m) in f16 (a weight is off by 2^-12 of itself, an
-//               eighth of the output's own rounding), each key's weight times its value scale
-//               relative to the group's largest, which multiplies the product in fp32
+//   O += V^T P  channels x queries, accumulated by the MMA; P in f16 (a weight is off by 2^-11 of
+//               itself at most, an eighth of the output's own rounding) is 2^(s - m) times the key's
+//               value scale over a reference, one for each block and query, that keeps the largest
+//               of them below 2^15.  The reference falls as m rises and rises when a weight would
+//               pass 2^15 (both move O by the same power of two), so that values however large take
+//               no precision from the others where their weight is nothing
 // Channels and keys map to fragment indices so that a lane reads consecutive bytes.  m is raised
-// only by a score more than 1 above it (the weights stay below 2, the f16 ones, times 2^14, below
-// 2^15): exact, as every term uses the same m.
+// only by a score more than 1 above it (a weight stays below 2): exact, as every term uses the same m.
 constexpr int kWarps = 4;
 constexpr int kQ = 8;                        // queries of a CTA
 constexpr int kGroup = 32;                   // keys of a group
@@ -419,11 +421,25 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     };
 
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // of queries 2t and 2t + 1
-    float o[2 * NB][4];
+    float o[2 * NB][4];                                     // in units of 1 / inv
+    float2 inv[NB];                                         // powers of two, one for each block and query
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) inv[k] = make_float2(__uint_as_float(254u << 23), __uint_as_float(254u << 23));
+    // O of block k, query c (0: 2t, 1: 2t + 1) in units of another inv, its exponent field moved by `by`
+    auto move = [&](int k, int c, float times, int by) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            o[2 * k + e][c] *= times;
+            o[2 * k + e][c + 2] *= times;
+        }
+        float& i = c == 0 ? inv[k].x : inv[k].y;
+        i = __uint_as_float(__float_as_uint(i) + ((uint32_t)by << 23));
+    };
+    auto field = [&](int k, int c) { return (int)(__float_as_uint(c == 0 ? inv[k].x : inv[k].y) >> 23); };
 
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i, i);
@@ -449,14 +465,13 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             __syncwarp();
         }
         // S = K Q^T: this lane has keys g + 8r of queries 2t and 2t + 1
-        float s[4][2];
-        float ksc[4][NB];
-        uint32_t vsw[4];
+        float2 s[4];
+        float ksc[4][NB], vsc[4][NB];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[r][0] = s[r][1] = 0.f;
+            s[r] = make_float2(0.f, 0.f);
             word_scales<NB>(scale_word<NB>(st + R::KS, g + 8 * r), ksc[r]);
-            vsw[r] = scale_word<NB>(st + R::VS, g + 8 * r);
+            word_scales<NB>(scale_word<NB>(st + R::VS, g + 8 * r), vsc[r]);
         }
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
@@ -471,20 +486,17 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
                 mma_f16(d, f0, q[k][0], q[k][1]);
                 mma_f16(d, f1, q[k][2], q[k][3]);
                 const float sa = ksc[2 * h][k], sb = ksc[2 * h + 1][k];
-                s[2 * h][0] = fmaf(d[0], sa, s[2 * h][0]);
-                s[2 * h][1] = fmaf(d[1], sa, s[2 * h][1]);
-                s[2 * h + 1][0] = fmaf(d[2], sb, s[2 * h + 1][0]);
-                s[2 * h + 1][1] = fmaf(d[3], sb, s[2 * h + 1][1]);
+                s[2 * h] = tc::ffma2v(make_float2(d[0], d[1]), make_float2(sa, sa), s[2 * h]);
+                s[2 * h + 1] = tc::ffma2v(make_float2(d[2], d[3]), make_float2(sb, sb), s[2 * h + 1]);
             }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[r][0] *= c0;
-            s[r][1] *= c1;
-            if (!whole && g + 8 * (r & 1) >= nl[r >> 1]) s[r][0] = s[r][1] = -INFINITY;
+            s[r] = fmul2(s[r], make_float2(c0, c1));
+            if (!whole && g + 8 * (r & 1) >= nl[r >> 1]) s[r] = make_float2(-INFINITY, -INFINITY);
         }
-        const float t0 = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
-        const float t1 = fmaxf(fmaxf(s[0][1], s[1][1]), fmaxf(s[2][1], s[3][1]));
+        const float t0 = fmaxf(fmaxf(s[0].x, s[1].x), fmaxf(s[2].x, s[3].x));
+        const float t1 = fmaxf(fmaxf(s[0].y, s[1].y), fmaxf(s[2].y, s[3].y));
         if (__any_sync(0xffffffffu, t0 > m0 + 1.f || t1 > m1 + 1.f)) {
             float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
 #pragma unroll
@@ -492,55 +504,63 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
                 n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, w));
                 n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, w));
             }
-            const float f0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
+            const float f[2] = {n0 == -INFINITY ? 1.f : exp2f(m0 - n0), n1 == -INFINITY ? 1.f : exp2f(m1 - n1)};
+            // whole powers of two by which m rises: the references follow (O only shrinks)
+            const int rise[2] = {(int)fminf(n0 - m0, 120.f), (int)fminf(n1 - m1, 120.f)};
             m0 = n0;
             m1 = n1;
-            l0 *= f0;
-            l1 *= f1;
+            l0 *= f[0];
+            l1 *= f[1];
 #pragma unroll
-            for (int j = 0; j < 2 * NB; ++j) {
-                o[j][0] *= f0;
-                o[j][1] *= f1;
-                o[j][2] *= f0;
-                o[j][3] *= f1;
-            }
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int by = min(254 - field(k, c), rise[c]);
+                    move(k, c, f[c] * __uint_as_float((uint32_t)(127 + by) << 23), by);
+                }
         }
         const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {                       // scores to weights
-            s[r][0] = exp2f(s[r][0] - r0);
-            s[r][1] = exp2f(s[r][1] - r1);
-            l0 += s[r][0];
-            l1 += s[r][1];
+            s[r] = make_float2(tc::ex2(s[r].x - r0), tc::ex2(s[r].y - r1));
+            l0 += s[r].x;
+            l1 += s[r].y;
         }
         // O += V^T P
-        // the group's largest value scales, of blocks 0, 2 and 1, 3 in the halves of two words
-        uint32_t top[2] = {0, 0};
+        uint32_t pk[NB][4];
+        auto weights = [&] {                                // of all blocks as f16 pairs; returns the largest
+            uint32_t top = 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            top[0] = __vmaxu2(top[0], vsw[r] & 0x00ff00ffu);
-            if (NB > 1) top[1] = __vmaxu2(top[1], (vsw[r] >> 8) & 0x00ff00ffu);
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float2 y = fmul2(fmul2(s[r], vsc[r][k]), inv[k]);
+                    pk[k][r] = pack_f16(y.x, y.y);
+                    top = __vmaxu2(top, pk[k][r]);
+                }
+            return max(top >> 16, top & 0xffffu);
+        };
+        if (__any_sync(0xffffffffu, weights() > 0x7800u)) {             // 2^15
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float w = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w = fmaxf(w, (c == 0 ? s[r].x : s[r].y) * vsc[r][k]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, x));
+                    // the exponent field that brings w to 2^13 ... 2^14
+                    const int by = max(267 - (int)(__float_as_uint(w) >> 23), 1) - field(k, c);
+                    if (by < 0) move(k, c, by > -127 ? __uint_as_float((uint32_t)(127 + by) << 23) : 0.f, by);
+                }
+            weights();
         }
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) {
-            top[0] = __vmaxu2(top[0], __shfl_xor_sync(0xffffffffu, top[0], w));
-            if (NB > 1) top[1] = __vmaxu2(top[1], __shfl_xor_sync(0xffffffffu, top[1], w));
-        }
-        float vsc[4][NB];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) word_scales<NB>(vsw[r], vsc[r]);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            // weights times 2^14 over the largest scale (2^127 at most), the product times its inverse
-            const int tk = k < 2 ? top[k & 1] & 255 : top[k & 1] >> 16 & 255;
-            const float inv = __uint_as_float((uint32_t)min(254, 268 - tk) << 23);
-            const float unit = __uint_as_float(max(max(tk - 14, 0) << 23, 0x00400000));
-            float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float fa = vsc[2 * h][k] * inv, fb = vsc[2 * h + 1][k] * inv;
-                const uint32_t b0 = transpose8(pack_f16(s[2 * h][0] * fa, s[2 * h][1] * fa));
-                const uint32_t b1 = transpose8(pack_f16(s[2 * h + 1][0] * fb, s[2 * h + 1][1] * fb));
+                const uint32_t b0 = transpose8(pk[k][2 * h]), b1 = transpose8(pk[k][2 * h + 1]);
                 uint32_t va[4], vb[4];                      // keys 2t, 2t + 1 and 2t + 8, 2t + 9 of the half
                 const uint8_t* v = st + R::V + (2 * t + 16 * h) * R::PITCH + (k * 32 + g * 4) * BITS / 8;
                 value_pairs<BITS>(v, v + R::PITCH, va);
@@ -548,13 +568,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t f[4] = {va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1]};
-                    mma_f16(d[e], f, b0, b1);
+                    mma_f16(o[2 * k + e], f, b0, b1);
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[2 * k + e][j] = fmaf(d[e][j], unit, o[2 * k + e][j]);
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -582,10 +598,16 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         x[3] = l1;
     }
 #pragma unroll
-    for (int j = 0; j < 2 * NB; ++j) {
-        float* x = so + (warp * kQ + 2 * t) * HD + j / 2 * 32 + g * 4 + (j & 1) * 2;
-        *reinterpret_cast<float2*>(x) = make_float2(o[j][0], o[j][2]);
-        *reinterpret_cast<float2*>(x + HD) = make_float2(o[j][1], o[j][3]);
+    for (int k = 0; k < NB; ++k) {
+        const float u0 = __uint_as_float(max((uint32_t)(254 - field(k, 0)) << 23, 0x00400000u));      // 1 / inv
+        const float u1 = __uint_as_float(max((uint32_t)(254 - field(k, 1)) << 23, 0x00400000u));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float* x = o[2 * k + e];
+            float* to = so + (warp * kQ + 2 * t) * HD + k * 32 + g * 4 + e * 2;
+            *reinterpret_cast<float2*>(to) = make_float2(x[0] * u0, x[2] * u0);
+            *reinterpret_cast<float2*>(to + HD) = make_float2(x[1] * u1, x[3] * u1);
+        }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < nq * HD; i += kWarps * 32) {

@@ -34,6 +34,16 @@ __device__ __forceinline__ float2 fmul2(float2 a, float s) {
     return o;
 }
 
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+    unsigned long long ra, rb, rd;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
+    asm("mov.b64 %0, {%1,%2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+    float2 o;
+    asm("mov.b64 {%0,%1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(rd));
+    return o;
+}
+
 // 16 consecutive elements (half a block) of a row as they are stored, their largest magnitude and
 // their values.  The 16-bit types' magnitudes are compared two at a time as integers.
 template <int T>

@@ -374,6 +374,31 @@ def test_attention_with_infinities_in_queries():
     check_attend(got[:, 96:], q[3:], c, _first_key_negative(k), v, t, [64], 8)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("order", ["first", "last", "each group"])
+def test_attention_huge_values_without_weight(order, bits):
+    """Values 2^90 times the others at keys whose weight is nothing beside the others': they must not
+    take the others' precision, whether they come first (with the largest score so far), last or
+    once in every group of keys; 300 sequences, so that a warp has several groups."""
+    g = gen(15 + bits)
+    c = fk.MxKvCache(125, 16, 2, 64, bits=bits, device=DEV)
+    n = c.slots
+    k = torch.randn(n, 128, generator=g, device=DEV).to(BF16)
+    v = torch.randn(n, 128, generator=g, device=DEV).to(BF16)
+    at = {"first": slice(0, 40), "last": slice(n - 40, n), "each group": slice(7, n, 32)}[order]
+    score = 700.0 if order == "each group" else torch.linspace(0, 700, n, device=DEV)[:, None]
+    k[:, ::64] = torch.as_tensor(score, device=DEV).to(BF16).expand(n, 2) if order != "last" else 700.0
+    k[at, ::64] = 0.0
+    v[at] = (v[at].float() * 2.0 ** 90).to(BF16)
+    fk.kv_cache_write(c, k, v, torch.arange(n, device=DEV))
+    q = torch.randn(300, 128, generator=g, device=DEV).to(BF16)
+    q[:, ::64] = 8.0                                          # scores up to 700 apart (scale 1/8)
+    t = torch.arange(125, dtype=torch.int32, device=DEV)[None].expand(300, 125)
+    got = fk.attention_1q_cached(q, c, t, i32([n] * 300))
+    for b in (0, 150, 299):
+        check_attend(got[b:b + 1], q[b:b + 1], c, k, v, t[b:b + 1], [n], bits)
+
+
 def _first_key_negative(k):
     k = k.clone()
     k[5, 0] = -1.0
