@@ -193,8 +193,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 // number of 16-byte chunks so that the fragment reads spread over the banks.  Per group and
 // 32-channel block:
 //   S = K Q^T   32 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
-//               query by a power of two that puts its largest channel at 2^13: exact but for
-//               channels 2^27 below that one
+//               query by a power of two that puts its largest channel at 2^15: exact but for
+//               channels 2^32 below that one
 //   O += V^T P  channels x queries, accumulated by the MMA; P in f16 (a weight is off by 2^-11 of
 //               itself at most, an eighth of the output's own rounding) is 2^(s - m) times the key's
 //               value scale over a reference, one for each block and query, that keeps the largest
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t e = top >> 23;
-        const uint32_t up = e == 0 || e == 255 ? 127u : min(253u, 267u - e);    // exponent field of the factor
+        const uint32_t up = e == 0 || e == 255 ? 127u : min(253u, 269u - e);    // exponent field of the factor
         const float unit = __uint_as_float((254u - up) << 23) * a.scale_log2;
         c0 = __shfl_sync(0xffffffffu, unit, 8 * t);
         c1 = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
