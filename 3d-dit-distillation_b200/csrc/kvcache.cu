@@ -4,7 +4,8 @@
 // Layout: slot = page * page_size + offset.  Keys (and, apart, values) are
 // [pages, heads, page_size, head_dim * bits / 8] bytes and their scales
 // [pages, heads, page_size, head_dim / 32] bytes, so the keys of one head in one page are
-// consecutive: what one query head reads.
+// consecutive: what one query head reads, in one copy of 16 keys.  The 16-byte pieces of a key are
+// exchanged (swapped_piece) so that this copy lands in shared memory without bank conflicts.
 #include <float.h>
 #include <math.h>
 
@@ -24,6 +25,7 @@ namespace {
 using namespace mx;
 
 constexpr int kErrIndex = 0x4B56;   // "KV": a slot, page or length outside the cache
+constexpr int kErrWait = 0x4B57;    // "KW": a bounded wait for copied keys ran out
 constexpr int kThreads = 256;
 constexpr int kMaxSplits = 1024;
 constexpr int64_t kMaxKeys = INT32_MAX - (1 << 20);          // of one sequence: positions stay int32
@@ -58,12 +60,21 @@ __device__ __forceinline__ void each_half(const Rows& r, F&& body) {
     }
 }
 
+// Which 16-byte piece of a key's row (of CH pieces) holds piece 0: piece p is at p ^ swapped_piece.
+// Eight neighbouring rows then have the same piece in different 16-byte columns of the 128 bytes
+// that shared memory's banks span.
+template <int CH>
+__host__ __device__ constexpr int swapped_piece(int row) {
+    return CH == 8 ? row & 7 : CH == 4 ? row >> 1 & 3 : CH == 6 || CH == 2 ? row >> 2 & 1 : 0;
+}
+
 // a thread's place in the cache
 template <int HD, int BITS>
 __device__ __forceinline__ void place(const Cache& c, int64_t slot, int ch, int64_t* data, int64_t* scale) {
     const int h = ch / HD, e = ch - h * HD;
     const int64_t at = ((slot >> c.page_shift) * c.heads + h) * c.page_size + (slot & (c.page_size - 1));
-    *data = at * (HD * BITS / 8) + e * BITS / 8;
+    constexpr int W = HD * BITS / 8;
+    *data = at * W + ((e * BITS / 8) ^ (swapped_piece<W / 16>((int)(slot & 7)) << 4));
     *scale = at * (HD / kBlock) + e / kBlock;
 }
 
@@ -189,8 +200,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 //
 // A CTA takes one sequence, one key head, up to 8 of its queries and a share ("split") of the keys.
 // Its warps are independent until the end: each takes groups of 32 consecutive keys (two halves of
-// 16, each in one page), copied by cp.async into the warp's own ring, rows padded to an odd
-// number of 16-byte chunks so that the fragment reads spread over the banks.  Per group and
+// 16, each in one page), copied by four bulk copies a half into the warp's own ring.  Per group and
 // 32-channel block:
 //   S = K Q^T   32 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
 //               query by a power of two that puts its largest channel at 2^15: exact but for
@@ -238,10 +248,6 @@ __device__ __forceinline__ float load_cluster(uint32_t addr, int rank) {
     float x;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::mapa_shared(addr, rank)));
     return x;
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -324,8 +330,7 @@ __device__ __forceinline__ void word_scales(uint32_t w, float* s) {
 template <int HD, int BITS>
 struct Ring {
     static constexpr int W = HD * BITS / 8, CH = W / 16, NB = HD / kBlock;
-    static constexpr int PITCH = CH % 2 ? W : W + 16;
-    static constexpr int V = kGroup * PITCH, KS = 2 * V, VS = KS + kGroup * NB, STAGE = VS + kGroup * NB;
+    static constexpr int V = kGroup * W, KS = 2 * V, VS = KS + kGroup * NB, STAGE = VS + kGroup * NB;
     // groups in the ring: what leaves room for three CTAs an SM, up to 4
     static constexpr int STAGES = 19000 / STAGE > 4 ? 4 : 19000 / STAGE;
     static_assert(STAGES >= 2, "");
@@ -341,11 +346,17 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float joined[kQ][2];                         // max and sum of the CTA's queries
     __shared__ int live[kWarps][kStages][2];                // keys that count of the halves of a group
+    __shared__ uint64_t full[kWarps][kStages];              // a group's copies have arrived
+    __shared__ int abort_flag;
     const int split = blockIdx.x, chunks = (a.group + kQ - 1) / kQ;
     const int kh = blockIdx.y / chunks, q0 = (blockIdx.y % chunks) * kQ, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nq = min(kQ, a.group - q0);
     asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x < kWarps * kStages) tc::mbar_init(tc::smem_u32(&full[0][0] + threadIdx.x), 1);
+    if (threadIdx.x == 0) abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
     constexpr int step = kWarps * kGroup;
     const int len = (int)length_of(a, c.page_size, b);      // an int32, as the caller's
     const int per = ((len + kGroup - 1) / kGroup + a.splits - 1) / a.splits * kGroup;
@@ -383,41 +394,32 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     uint8_t* ring = smem + warp * R::WARP;
     const int32_t* table = a.table + b * a.ldt;
     int pages = -1;                                         // lane j: page of half j of 16 groups
-    auto issue = [&](int i, int s) {                        // copy group i of this warp, if there is one, to stage s
-        if (i < mine) {
-            if ((i & 15) == 0) {
-                const int j = first + (i + (lane >> 1)) * step + (lane & 1) * 16;
-                pages = j < end ? __ldg(table + (j >> c.page_shift)) : -1;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int page = __shfl_sync(0xffffffffu, pages, (i & 15) * 2 + h);
-                const int key = first + i * step + h * 16;
-                const bool there = key < end && page >= 0 && page < c.pages;
-                if (lane == 0) {
-                    live[warp][s][h] = there ? min(16, end - key) : 0;
-                    if (key < end && !there) atomicExch(&g_kvcache_error, kErrIndex);
-                }
-                if (!there) continue;
+    // copy group i of this warp, if there is one, to stage s: lanes 0 and 1 a half each
+    auto issue = [&](int i, int s) {
+        if (i >= mine) return;
+        if ((i & 15) == 0) {
+            const int j = first + (i + (lane >> 1)) * step + (lane & 1) * 16;
+            pages = j < end ? __ldg(table + (j >> c.page_shift)) : -1;
+        }
+        const int h = lane & 1, page = __shfl_sync(0xffffffffu, pages, (i & 15) * 2 + h);
+        const int key = first + i * step + h * 16;
+        const bool there = key < end && page >= 0 && page < c.pages;
+        const uint32_t halves = __popc(__ballot_sync(0xffffffffu, lane < 2 && there));
+        const uint32_t bar = tc::smem_u32(&full[warp][s]);
+        if (lane == 0) tc::mbar_expect_tx(bar, halves * (16 * 2 * (R::W + NB)));
+        if (lane < 2) {
+            live[warp][s][h] = there ? min(16, end - key) : 0;
+            if (there) {
                 const int64_t row = ((int64_t)page * c.heads + kh) * c.page_size + (key & (c.page_size - 1));
-                const uint32_t dst = tc::smem_u32(ring + s * R::STAGE) + h * 16 * R::PITCH;
-                const uint8_t *ks = c.k + row * R::W, *vs = c.v + row * R::W;
-#pragma unroll
-                for (int j = 0; j < (16 * R::CH + 31) / 32; ++j) {
-                    const int chunk = lane + 32 * j;
-                    if (16 * R::CH % 32 == 0 || chunk < 16 * R::CH) {
-                        const uint32_t to = dst + chunk / R::CH * R::PITCH + chunk % R::CH * 16;
-                        cp_async16(to, ks + chunk * 16);
-                        cp_async16(to + R::V, vs + chunk * 16);
-                    }
-                }
-                const int part = lane & 15;
-                if (part < NB)
-                    cp_async16(tc::smem_u32(ring + s * R::STAGE) + (lane < 16 ? R::KS : R::VS) + (h * NB + part) * 16,
-                               (lane < 16 ? c.ks : c.vs) + row * NB + part * 16);
+                const uint32_t dst = tc::smem_u32(ring + s * R::STAGE);
+                tc::bulk_load(dst + h * 16 * R::W, c.k + row * R::W, 16 * R::W, bar);
+                tc::bulk_load(dst + R::V + h * 16 * R::W, c.v + row * R::W, 16 * R::W, bar);
+                tc::bulk_load(dst + R::KS + h * 16 * NB, c.ks + row * NB, 16 * NB, bar);
+                tc::bulk_load(dst + R::VS + h * 16 * NB, c.vs + row * NB, 16 * NB, bar);
+            } else if (key < end) {
+                atomicExch(&g_kvcache_error, kErrIndex);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // of queries 2t and 2t + 1
@@ -443,25 +445,36 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i, i);
+    // where in a row this lane's 8 channels of a key and 4 of a value are: within the piece, and the
+    // exchange of pieces in its rows (g + 8r; 2t + 8r and the next)
+    const int key_at = BITS == 8 ? (t & 1) * 8 : t * 4, value_at = BITS == 8 ? (g & 3) * 4 : g * 2;
+    const int key_swap = ((BITS == 8 ? t >> 1 : 0) ^ swapped_piece<R::CH>(g)) << 4;
+    const int value_swap[2] = {((BITS == 8 ? g >> 2 : 0) ^ swapped_piece<R::CH>(2 * t)) << 4,
+                               ((BITS == 8 ? g >> 2 : 0) ^ swapped_piece<R::CH>(2 * t + 1)) << 4};
     int seen = 0;                                           // whether any key of this warp counted
     int cur = 0, next = kStages - 1;                        // the stage of this step and the one its copies go to
+    uint32_t phase = 0;                                     // of the stages' barriers
     for (int i = 0; i < mine; ++i) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        __syncwarp();
-        issue(i + kStages - 1, next);                       // the stage the last step has read
+        __syncwarp();                                       // every lane has read the stage that is filled next
+        issue(i + kStages - 1, next);
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&full[warp][cur]), phase, &abort_flag, &g_kvcache_error,
+                                                   kErrWait)))
+            break;
         uint8_t* st = ring + cur * R::STAGE;
         const int nl[2] = {live[warp][cur][0], live[warp][cur][1]};
         next = cur;
         cur = cur == kStages - 1 ? 0 : cur + 1;
+        if (cur == 0) phase ^= 1;
         const bool whole = nl[0] + nl[1] == kGroup;
         seen |= nl[0] + nl[1];
         if (!whole) {
             // keys that do not count: their values and scales, whatever is there, must not reach the sums
             for (int r = 0; r < kGroup; ++r) {
                 if ((r & 15) < nl[r >> 4]) continue;
-                for (int j = lane; j < R::W / 4; j += 32) *reinterpret_cast<uint32_t*>(st + R::V + r * R::PITCH + j * 4) = 0;
+                for (int j = lane; j < R::W / 4; j += 32) *reinterpret_cast<uint32_t*>(st + R::V + r * R::W + j * 4) = 0;
                 if (lane < NB) st[R::VS + r * NB + lane] = 0;
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before a later copy to the stage
             __syncwarp();
         }
         // S = K Q^T: this lane has keys g + 8r of queries 2t and 2t + 1
@@ -478,9 +491,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t ka[4], kb[4];
-                const uint8_t* p = st + (g + 16 * h) * R::PITCH + (k * 32 + t * 8) * BITS / 8;
+                const uint8_t* p = st + (g + 16 * h) * R::W + ((k * 4 * BITS) ^ key_swap) + key_at;
                 key_pairs<BITS>(p, ka);
-                key_pairs<BITS>(p + 8 * R::PITCH, kb);
+                key_pairs<BITS>(p + 8 * R::W, kb);
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
                 const uint32_t f0[4] = {ka[0], kb[0], ka[1], kb[1]}, f1[4] = {ka[2], kb[2], ka[3], kb[3]};
                 mma_f16(d, f0, q[k][0], q[k][1]);
@@ -562,9 +575,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             for (int h = 0; h < 2; ++h) {
                 const uint32_t b0 = transpose8(pk[k][2 * h]), b1 = transpose8(pk[k][2 * h + 1]);
                 uint32_t va[4], vb[4];                      // keys 2t, 2t + 1 and 2t + 8, 2t + 9 of the half
-                const uint8_t* v = st + R::V + (2 * t + 16 * h) * R::PITCH + (k * 32 + g * 4) * BITS / 8;
-                value_pairs<BITS>(v, v + R::PITCH, va);
-                value_pairs<BITS>(v + 8 * R::PITCH, v + 9 * R::PITCH, vb);
+                const uint8_t* v = st + R::V + (2 * t + 16 * h) * R::W + value_at;
+                const uint8_t *v0 = v + ((k * 4 * BITS) ^ value_swap[0]), *v1 = v + R::W + ((k * 4 * BITS) ^ value_swap[1]);
+                value_pairs<BITS>(v0, v1, va);
+                value_pairs<BITS>(v0 + 8 * R::W, v1 + 8 * R::W, vb);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t f[4] = {va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1]};
@@ -573,8 +587,6 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             }
         }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-
     // a warp whose scores were all -inf (a query with infinities) has seen keys, unlike an empty one:
     // alone it makes 0 / 0, not zeros
     if (seen) {

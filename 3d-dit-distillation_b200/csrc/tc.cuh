@@ -460,6 +460,13 @@ __device__ __forceinline__ void tc_mxf4_step_elect(uint32_t d_tmem, uint64_t a_d
             : "memory");
 }
 
+// untiled bulk copy (16-byte aligned, a multiple of 16 bytes) counted on an mbarrier of this CTA
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link)
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
 

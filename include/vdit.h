@@ -358,7 +358,9 @@ int vdit_linear_mxfp4_dense(const void* x, int32_t x_type, int64_t ldx, const vo
 /* A paged cache of keys and values in a microscaled format, bits 8 (e4m3) or 4 (e2m1).  Slot
  * page * page_size + offset holds one row of heads * head_dim channels: k and v are
  * [pages, heads, page_size, head_dim * bits / 8] bytes, k_scales and v_scales
- * [pages, heads, page_size, head_dim / 32] bytes, device memory of the caller's, 16-byte aligned.
+ * [pages, heads, page_size, head_dim / 32] bytes, device memory of the caller's, 16-byte aligned
+ * (the 16-byte pieces of a key's data stand in an order of the library's own: fill and read the
+ * cache through these entry points).
  * page_size is a power of two from 16 to 1024; head_dim 32, 64, 96 or 128.  The struct itself is
  * host memory, read during the call. */
 typedef struct vdit_kv_cache {

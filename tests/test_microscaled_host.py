@@ -135,16 +135,29 @@ def test_c_entry_points_check_before_any_launch():
 @pytest.mark.parametrize("pages,page,heads,hd,bits", [(3, 16, 5, 96, 4), (7, 16, 2, 32, 8), (2, 1024, 3, 128, 8),
                                                        (70000, 128, 12, 128, 8)])
 def test_cache_addresses_stay_inside_and_apart(pages, page, heads, hd, bits):
-    """The kernels' address arithmetic, ((page * heads + head) * page_size + offset) * width + element
-    bytes: the last 16 channels of the last slot end where the buffer ends (past 2^32 bytes in the
-    last case), and no two (slot, head) overlap."""
+    """The kernels' address arithmetic, ((page * heads + head) * page_size + offset) * width + the byte of
+    the channels with its 16-byte piece exchanged: the last slot ends where the buffer ends (past 2^32
+    bytes in the last case), no two pieces share bytes, and the 16 keys of a copy are consecutive and
+    16-byte aligned."""
     width, nb = hd * bits // 8, pages * heads * page * (hd * bits // 8)
-    last = ((np.int64(pages - 1) * heads + heads - 1) * page + page - 1) * width + (hd - 16) * bits // 8
-    assert last + 16 * bits // 8 == nb
+    pieces = width // 16
+
+    def swap(row):
+        return {8: row & 7, 4: row >> 1 & 3, 6: row >> 2 & 1, 2: row >> 2 & 1}.get(pieces, row & 0)
+
+    last = ((np.int64(pages - 1) * heads + heads - 1) * page + page - 1) * width
+    assert last + width == nb
+    row, p = np.meshgrid(np.arange(16), np.arange(pieces), indexing="ij")
+    at = row * width + ((p * 16) ^ (swap(row) * 16))
+    assert np.array_equal(np.sort(at.ravel()), np.arange(16 * pieces) * 16)     # a permutation within the copy
+    assert all(set(at[r] // width) == {r} for r in range(16))                   # and within each row
+    # eight neighbouring rows have the same piece in 8 of the 128 bytes' 16-byte columns, or all they can
+    for q in range(pieces):
+        assert len(set(at[:8, q] // 16 % 8)) == 8
     if pages < 100:
-        p, h, o = np.meshgrid(np.arange(pages), np.arange(heads), np.arange(page), indexing="ij")
-        at = ((p * heads + h) * page + o) * width
-        assert len(np.unique(at)) == at.size and at.max() + width == nb
+        pg, h, o = np.meshgrid(np.arange(pages), np.arange(heads), np.arange(0, page, 16), indexing="ij")
+        start = ((pg * heads + h) * page + o) * width
+        assert len(np.unique(start)) == start.size and (start % 16 == 0).all() and start.max() + 16 * width == nb
 
 
 def test_runner_refuses_unknown_four_bit_linears():
