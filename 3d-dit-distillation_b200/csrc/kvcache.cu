@@ -230,7 +230,7 @@ struct AttnArgs {
     int splits;                              // key ranges of a sequence
     int cluster;                             // CTAs of a cluster: 1, or all splits of a sequence and head
     float scale_log2;
-    float* ws;                               // [batch, heads, splits, 2 + hd] when splits > 1
+    float* ws;                               // [batch, heads, splits, 2 + hd] when not in a cluster
 };
 
 // a sequence's length, held inside its table row
