@@ -90,9 +90,10 @@ __device__ __forceinline__ void put_half(const Half<VDIT_BF16>& x, uint8_t* data
 }
 
 template <int HD, int BITS>
-__global__ void __launch_bounds__(kThreads) write_kernel(const __nv_bfloat16* __restrict__ k, int64_t ldk,
-                                                         const __nv_bfloat16* __restrict__ v, int64_t ldv,
-                                                         const int64_t* __restrict__ slots, Rows r, Cache c) {
+__global__ void __launch_bounds__(kThreads) write_kernel(const __nv_bfloat16* k, int64_t ldk,
+                                                         const __nv_bfloat16* v, int64_t ldv,
+                                                         const int64_t* slots, Rows r, Cache c) {
+    after_previous();
     each_half(r, [&](int64_t row0, int apart, int ch) {
         int64_t slot[kRowsAtOnce];
         Half<VDIT_BF16> a[kRowsAtOnce], b[kRowsAtOnce];
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __nv_bfloat16* __
             const int64_t row = row0 + u * apart;
             slot[u] = -1;
             if (row < r.n) {
-                slot[u] = __ldg(slots + row);
+                slot[u] = load_after(slots + row);
                 a[u].load(k + row * ldk + ch);
                 b[u].load(v + row * ldv + ch);
             }
@@ -127,13 +128,13 @@ struct HalfCodes {
     uint32_t s;
     __device__ __forceinline__ void load(const uint8_t* data, const uint8_t* scale) {
         if (BITS == 8) {
-            u = __ldg(reinterpret_cast<const uint4*>(data));
+            u = load_after(reinterpret_cast<const uint4*>(data));
         } else {
-            const uint2 t = __ldg(reinterpret_cast<const uint2*>(data));
+            const uint2 t = load_after(reinterpret_cast<const uint2*>(data));
             u.x = t.x;
             u.y = t.y;
         }
-        s = __ldg(scale);
+        s = load_after(scale);
     }
     template <typename T>
     __device__ __forceinline__ void store(T* out) const {
@@ -160,14 +161,15 @@ struct HalfCodes {
 };
 
 template <int HD, int BITS, typename T>
-__global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* __restrict__ slots, Rows r,
+__global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* slots, Rows r,
                                                         T* __restrict__ k, int64_t ldk, T* __restrict__ v,
                                                         int64_t ldv) {
+    after_previous();
     each_half(r, [&](int64_t row0, int apart, int ch) {
         int64_t slot[kRowsAtOnce];
         HalfCodes<BITS> a[kRowsAtOnce], b[kRowsAtOnce];
 #pragma unroll
-        for (int u = 0; u < kRowsAtOnce; ++u) slot[u] = row0 + u * apart < r.n ? __ldg(slots + row0 + u * apart) : -1;
+        for (int u = 0; u < kRowsAtOnce; ++u) slot[u] = row0 + u * apart < r.n ? load_after(slots + row0 + u * apart) : -1;
 #pragma unroll
         for (int u = 0; u < kRowsAtOnce; ++u) {
             a[u] = b[u] = HalfCodes<BITS>{make_uint4(0, 0, 0, 0), 0};
@@ -235,7 +237,7 @@ struct AttnArgs {
 
 // a sequence's length, held inside its table row
 __device__ __forceinline__ int64_t length_of(const AttnArgs& a, int page_size, int b) {
-    const int64_t most = (int64_t)a.max_pages * page_size, n = __ldg(a.lengths + b);
+    const int64_t most = (int64_t)a.max_pages * page_size, n = load_after(a.lengths + b);
     if (n < 0 || n > most) {
         atomicExch(&g_kvcache_error, kErrIndex);
         return n < 0 ? 0 : most;
@@ -352,12 +354,12 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     const int kh = blockIdx.y / chunks, q0 = (blockIdx.y % chunks) * kQ, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nq = min(kQ, a.group - q0);
-    asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x < kWarps * kStages) tc::mbar_init(tc::smem_u32(&full[0][0] + threadIdx.x), 1);
     if (threadIdx.x == 0) abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
     constexpr int step = kWarps * kGroup;
+    after_previous();
     const int len = (int)length_of(a, c.page_size, b);      // an int32, as the caller's
     const int per = ((len + kGroup - 1) / kGroup + a.splits - 1) / a.splits * kGroup;
     const int first = (int)min((int64_t)len, (int64_t)split * per) + warp * kGroup;   // groups at first + i * step ...
@@ -374,7 +376,16 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         for (int i = 0; i < NB; ++i) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-            if (g < nq) load8(a.q + b * a.ldq + (int64_t)(kh * a.group + q0 + g) * HD + i * 32 + t * 8, f[i]);
+            if (g < nq) {
+                const uint4 u = load_after(reinterpret_cast<const uint4*>(
+                    a.q + b * a.ldq + (int64_t)(kh * a.group + q0 + g) * HD + i * 32 + t * 8));
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f[i][2 * j] = __uint_as_float(w[j] << 16);
+                    f[i][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                }
+            }
             top = max(top, amax8(f[i]));
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -399,7 +410,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         if (i >= mine) return;
         if ((i & 15) == 0) {
             const int j = first + (i + (lane >> 1)) * step + (lane & 1) * 16;
-            pages = j < end ? __ldg(table + (j >> c.page_shift)) : -1;
+            pages = j < end ? load_after(table + (j >> c.page_shift)) : -1;
         }
         const int h = lane & 1, page = __shfl_sync(0xffffffffu, pages, (i & 15) * 2 + h);
         const int key = first + i * step + h * 16;
@@ -749,31 +760,28 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
         return VDIT_ERR_LAUNCH;
     }
     const dim3 grid(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (a.cluster > 1) {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = a.cluster;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.gridDim = grid;
-        cfg.blockDim = dim3(kWarps * 32);
-        cfg.dynamicSmemBytes = bytes;
-        e = cudaLaunchKernelEx(&cfg, attend_kernel<HD, BITS>, c, a);
-        if (e != cudaSuccess) {
-            record_cuda_error(e);
-            return VDIT_ERR_LAUNCH;
-        }
-    } else {
-        attend_kernel<HD, BITS><<<grid, kWarps * 32, bytes, s>>>(c, a);
+    cfg.numAttrs = a.cluster > 1 ? 2 : 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = bytes;
+    e = cudaLaunchKernelEx(&cfg, attend_kernel<HD, BITS>, c, a);
+    if (e != cudaSuccess) {
+        record_cuda_error(e);
+        return VDIT_ERR_LAUNCH;
     }
     count_launches(1);
     if (a.splits > a.cluster) {
         // resident before the splits are done: the launch is hidden behind them
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
         cfg.gridDim = dim3(a.heads, batch);
         cfg.blockDim = dim3(HD);
         cfg.dynamicSmemBytes = 0;
@@ -858,8 +866,8 @@ extern "C" int vdit_kv_cache_write(const void* k, int64_t ldk, const void* v, in
     if (!ctas) return VDIT_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     with_format(c.hd, cache->bits, [&](auto hd, auto bits) {
-        write_kernel<decltype(hd)::value, decltype(bits)::value><<<(unsigned)ctas, threads, 0, s>>>(
-            static_cast<const __nv_bfloat16*>(k), ldk, static_cast<const __nv_bfloat16*>(v), ldv, slots, r, c);
+        launch_early(write_kernel<decltype(hd)::value, decltype(bits)::value>, dim3((unsigned)ctas), threads, s,
+                     static_cast<const __nv_bfloat16*>(k), ldk, static_cast<const __nv_bfloat16*>(v), ldv, slots, r, c);
     });
     count_launches(1);
     return check_launch();
@@ -884,11 +892,11 @@ extern "C" int vdit_kv_cache_read(const vdit_kv_cache* cache, const int64_t* slo
     with_format(c.hd, cache->bits, [&](auto hd, auto bits) {
         constexpr int HD = decltype(hd)::value, BITS = decltype(bits)::value;
         if (out_type == VDIT_F32)
-            read_kernel<HD, BITS><<<(unsigned)ctas, threads, 0, s>>>(c, slots, r, static_cast<float*>(k), ldk,
-                                                                    static_cast<float*>(v), ldv);
+            launch_early(read_kernel<HD, BITS, float>, dim3((unsigned)ctas), threads, s, c, slots, r,
+                         static_cast<float*>(k), ldk, static_cast<float*>(v), ldv);
         else
-            read_kernel<HD, BITS><<<(unsigned)ctas, threads, 0, s>>>(c, slots, r, static_cast<__nv_bfloat16*>(k), ldk,
-                                                                    static_cast<__nv_bfloat16*>(v), ldv);
+            launch_early(read_kernel<HD, BITS, __nv_bfloat16>, dim3((unsigned)ctas), threads, s, c, slots, r,
+                         static_cast<__nv_bfloat16*>(k), ldk, static_cast<__nv_bfloat16*>(v), ldv);
     });
     count_launches(1);
     return check_launch();

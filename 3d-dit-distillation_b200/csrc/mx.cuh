@@ -44,14 +44,57 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
     return o;
 }
 
+// Waits until the kernels before this one in the stream are complete and what they wrote is visible,
+// then lets the next one set itself up.  In this order: when the next kernel starts, only this one is
+// still running, so that neither waits pile up nor a bounded wait there counts an older kernel's time.
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Loads of what an earlier kernel may have written while this one was already there: not read-only for
+// this kernel's whole life, so not through the read-only path (__ldg), and never moved above the wait.
+__device__ __forceinline__ uint4 load_after(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 load_after(const uint2* p) {
+    uint2 v;
+    asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load_after(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ int64_t load_after(const int64_t* p) {
+    int64_t v;
+    asm volatile("ld.global.b64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ int32_t load_after(const int32_t* p) {
+    int32_t v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t load_after(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
 // 16 consecutive elements (half a block) of a row as they are stored, their largest magnitude and
 // their values.  The 16-bit types' magnitudes are compared two at a time as integers.
 template <int T>
 struct Half {
     uint4 u[2];
     __device__ __forceinline__ void load(const void* p) {
-        u[0] = __ldg(static_cast<const uint4*>(p));
-        u[1] = __ldg(static_cast<const uint4*>(p) + 1);
+        u[0] = load_after(static_cast<const uint4*>(p));
+        u[1] = load_after(static_cast<const uint4*>(p) + 1);
     }
     __device__ __forceinline__ void zero() { u[0] = u[1] = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ uint32_t word(int i) const {
@@ -76,7 +119,7 @@ struct Half<VDIT_F32> {
     float4 u[4];
     __device__ __forceinline__ void load(const void* p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = __ldg(static_cast<const float4*>(p) + i);
+        for (int i = 0; i < 4; ++i) u[i] = load_after(static_cast<const float4*>(p) + i);
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -260,6 +303,24 @@ __device__ __forceinline__ void decode4_e4m3(uint32_t c, __half2* h) {
         : "r"(c));
 #pragma unroll
     for (int i = 0; i < 2; ++i) h[i] = *reinterpret_cast<__half2*>(&r[i]);
+}
+
+// A launch that may be set up while the kernel before it in the stream ends; the kernel calls
+// after_previous() in every thread before it touches global memory.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t s, Args... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+    if (e != cudaSuccess) record_cuda_error(e);             // check_launch() then reports it, too
+    return e;
 }
 
 // The scales of a quantised matrix [rows, cols] are held in the order the block-scaled MMA

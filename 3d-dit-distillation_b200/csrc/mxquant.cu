@@ -32,10 +32,10 @@ __device__ __forceinline__ Place place_of(int groups, int* group) {
 }
 
 template <int T>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const typename Elem<T>::type* __restrict__ x, int64_t ldx,
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const typename Elem<T>::type* x, int64_t ldx,
                                                             int64_t rows, int cols, int groups,
                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    asm volatile("griddepcontrol.launch_dependents;");      // a product of this matrix may set itself up meanwhile
+    after_previous();                                       // a product of this matrix may then set itself up
     int g;
     const Place at = place_of(groups, &g);
     if (g >= groups) return;                                // whole warps leave
@@ -63,20 +63,21 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const typename Elem<
 }
 
 template <int T>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes,
-                                                              const uint8_t* __restrict__ scales, int64_t rows,
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* codes,
+                                                              const uint8_t* scales, int64_t rows,
                                                               int cols, int groups,
                                                               typename Elem<T>::type* __restrict__ out, int64_t ldo) {
+    after_previous();
     int g;
     const Place at = place_of(groups, &g);
     if (g >= groups || at.col >= cols) return;
-    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(scales + at.scale));
+    const uint4 sw = load_after(reinterpret_cast<const uint4*>(scales + at.scale));
     const uint32_t word[4] = {sw.x, sw.y, sw.z, sw.w};
     uint2 c[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         c[i] = at.row + 32 * i < rows
-                   ? __ldg(reinterpret_cast<const uint2*>(codes + (at.row + 32 * i) * (cols / 2) + at.col / 2))
+                   ? load_after(reinterpret_cast<const uint2*>(codes + (at.row + 32 * i) * (cols / 2) + at.col / 2))
                    : make_uint2(0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -137,8 +138,8 @@ extern "C" int vdit_mxfp4_quantize(const void* x, int32_t x_type, int64_t ldx, i
     const int groups = scale_col_groups(cols);
     auto run = [&](auto tag) {
         constexpr int T = decltype(tag)::value;
-        quantize_kernel<T><<<grid, kThreads, 0, s>>>(static_cast<const typename Elem<T>::type*>(x), ldx, rows, cols, groups,
-                                                     static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
+        launch_early(quantize_kernel<T>, grid, kThreads, s, static_cast<const typename Elem<T>::type*>(x), ldx, rows, cols,
+                     groups, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
     };
     if (x_type == VDIT_BF16) run(std::integral_constant<int, VDIT_BF16>{});
     else if (x_type == VDIT_F16) run(std::integral_constant<int, VDIT_F16>{});
@@ -159,9 +160,9 @@ extern "C" int vdit_mxfp4_dequantize(const void* codes, const void* scales, int6
     const int groups = scale_col_groups(cols);
     auto run = [&](auto tag) {
         constexpr int T = decltype(tag)::value;
-        dequantize_kernel<T><<<grid, kThreads, 0, s>>>(
-            static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, cols, groups,
-            static_cast<typename Elem<T>::type*>(out), ldo);
+        launch_early(dequantize_kernel<T>, grid, kThreads, s, static_cast<const uint8_t*>(codes),
+                     static_cast<const uint8_t*>(scales), rows, cols, groups,
+                     static_cast<typename Elem<T>::type*>(out), ldo);
     };
     if (out_type == VDIT_BF16) run(std::integral_constant<int, VDIT_BF16>{});
     else if (out_type == VDIT_F16) run(std::integral_constant<int, VDIT_F16>{});

@@ -554,6 +554,78 @@ def test_captured_and_on_another_stream():
             assert all(torch.equal(a, b) for a, b in zip(got, w))
 
 
+@pytest.mark.parametrize("rows", [3, 700, 9000])
+def test_each_call_waits_for_the_one_before(rows):
+    """Every call reads what the call before it wrote (a kernel, a copy or another stream's kernel), in
+    place and on the same buffers each time, eagerly and captured: as with a wait on the host between."""
+    g = gen(31)
+    heads, hd, page, d = 2, 64, 64, 128
+    xs = torch.randn(6, rows, d, generator=g, device=DEV).to(BF16)
+    wq = fk.quantize_mxfp4(torch.randn(256, d, generator=g, device=DEV).to(BF16))
+    perm = torch.randperm(rows, generator=g, device=DEV)
+    pages = -(-rows // page)
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).flip(0).contiguous()[None]
+    side = torch.cuda.Stream()
+
+    def chain(b, bias, sync):
+        out = []
+        for i in range(xs.shape[0]):
+            wait = torch.cuda.synchronize if sync else (lambda: None)
+            b["x"].copy_(xs[i])
+            wait()
+            r = fk.dequantize_mxfp4(fk.quantize_mxfp4(b["x"]), dtype=BF16)
+            wait()
+            fk.kv_cache_write(b["c"], r, b["x"], b["slots"])
+            wait()
+            k, v = fk.kv_cache_read(b["c"], b["slots"])
+            wait()
+            b["slots"].copy_(perm[b["slots"]])               # the next write goes elsewhere
+            wait()
+            fk.kv_cache_write(b["c"], v, k, b["slots"])
+            wait()
+            o = fk.attention_1q_cached(k[:1], b["c"], table, b["n"])
+            wait()
+            fork = torch.cuda.current_stream()
+            side.wait_stream(fork)
+            with torch.cuda.stream(side):
+                y = fk.linear_mxfp4(v, wq, bias)
+            fork.wait_stream(side)
+            wait()
+            b["x"].copy_(y[:, :d])
+            wait()
+            q = fk.quantize_mxfp4(b["x"])
+            wait()
+            z = fk.linear_mxfp4(q, wq, y[0])                 # its bias is a product's row
+            wait()
+            b["n"].sub_(1).clamp_(min=1)
+            out += [r, k, v, o, y, z]
+        return out
+
+    def fresh():
+        return {"x": torch.empty(rows, d, dtype=BF16, device=DEV), "slots": torch.arange(rows, device=DEV),
+                "c": fk.MxKvCache(pages, page, heads, hd, device=DEV), "n": i32([rows])}
+
+    bias = torch.randn(256, generator=g, device=DEV).to(BF16)
+    want = chain(fresh(), bias, True)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = chain(fresh(), bias, False)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(got, want))
+    b, graph = fresh(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(b, bias, False)
+    for _ in range(5):
+        start = fresh()
+        b["slots"].copy_(start["slots"])
+        b["n"].copy_(start["n"])
+        for name in ("k", "v", "k_scales", "v_scales"):
+            getattr(b["c"], name).copy_(getattr(start["c"], name))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(got, want))
+
+
 # ----------------------------------------------------------------------------- on the model's path
 
 def _model(dim=256, depth=3, cond_depth=2, n=700, side=8):
