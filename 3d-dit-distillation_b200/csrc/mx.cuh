@@ -307,6 +307,8 @@ __device__ __forceinline__ void decode4_e4m3(uint32_t c, __half2* h) {
 
 // A launch that may be set up while the kernel before it in the stream ends; the kernel calls
 // after_previous() in every thread before it touches global memory.
+// It saves the gap between two calls of a stream, 1.5 to 2 us a launch (quantise and read back 7680 x 1536:
+// 26.4 -> 21.5 us; write and read back 4101 rows of 12 x 128: 21.5 -> 17.2), not time of the kernels.
 template <typename... Params, typename... Args>
 inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t s, Args... args) {
     cudaLaunchAttribute attr[1];

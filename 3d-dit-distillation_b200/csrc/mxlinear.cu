@@ -167,7 +167,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (every CTA)
         if (lane == 0) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");          // a is written (when launched beside its writer)
+            // a is written, when launched beside its writer.  That one lets this kernel start only after
+            // its own wait, so all older kernels are complete: the epilogue reads the bias without a wait.
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             int it = 0;
             bool ok = true;
             for (int t = unit; ok && t < ntiles; t += nunits) {

@@ -597,8 +597,14 @@ def test_each_call_waits_for_the_one_before(rows):
             wait()
             z = fk.linear_mxfp4(q, wq, y[0])                 # its bias is a product's row
             wait()
+            rows_q = fk.quantize_mxfp4(y)
+            wait()
+            row = fk.dequantize_mxfp4(rows_q, dtype=BF16)[0]
+            wait()
+            u = fk.linear_mxfp4(b["x"], wq, row)             # its bias is the last call's
+            wait()
             b["n"].sub_(1).clamp_(min=1)
-            out += [r, k, v, o, y, z]
+            out += [r, k, v, o, y, z, u]
         return out
 
     def fresh():
