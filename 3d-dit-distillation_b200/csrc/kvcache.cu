@@ -236,8 +236,8 @@ struct AttnArgs {
 };
 
 // a sequence's length, held inside its table row
-__device__ __forceinline__ int64_t length_of(const AttnArgs& a, int page_size, int b) {
-    const int64_t most = (int64_t)a.max_pages * page_size, n = load_after(a.lengths + b);
+__device__ __forceinline__ int64_t length_of(const AttnArgs& a, int page_size, int64_t n) {
+    const int64_t most = (int64_t)a.max_pages * page_size;
     if (n < 0 || n > most) {
         atomicExch(&g_kvcache_error, kErrIndex);
         return n < 0 ? 0 : most;
@@ -360,7 +360,15 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     __syncthreads();
     constexpr int step = kWarps * kGroup;
     after_previous();
-    const int len = (int)length_of(a, c.page_size, b);      // an int32, as the caller's
+    // the query is loaded before the branch on the length, so that the two latencies pass at once
+    const int32_t given = load_after(a.lengths + b);
+    uint4 raw[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+        raw[i] = g < nq ? load_after(reinterpret_cast<const uint4*>(
+                              a.q + b * a.ldq + (int64_t)(kh * a.group + q0 + g) * HD + i * 32 + t * 8))
+                        : make_uint4(0, 0, 0, 0);
+    const int len = (int)length_of(a, c.page_size, given);      // an int32, as the caller's
     const int per = ((len + kGroup - 1) / kGroup + a.splits - 1) / a.splits * kGroup;
     const int first = (int)min((int64_t)len, (int64_t)split * per) + warp * kGroup;   // groups at first + i * step ...
     const int end = (int)min((int64_t)len, (int64_t)(split + 1) * per);               // ... below end
@@ -374,17 +382,11 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[i][j] = 0.f;
-            if (g < nq) {
-                const uint4 u = load_after(reinterpret_cast<const uint4*>(
-                    a.q + b * a.ldq + (int64_t)(kh * a.group + q0 + g) * HD + i * 32 + t * 8));
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f[i][2 * j] = __uint_as_float(w[j] << 16);
-                    f[i][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                }
+            for (int j = 0; j < 4; ++j) {
+                f[i][2 * j] = __uint_as_float(w[j] << 16);
+                f[i][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
             }
             top = max(top, amax8(f[i]));
         }
@@ -725,7 +727,7 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
 // for an even end, where a split then still has 1024.  Where up to 16 splits that all run at once have
 // no more than 2048 keys each, they are a cluster, which joins them itself (one launch, no workspace);
 // otherwise their states go through the workspace to a second kernel (16 sequences of up to 32768
-// keys: 200 us, in clusters of 2 or 8 272 and 233).
+// keys: 200 us when this was chosen, 183 now; in clusters of 2 or 8 272 and 233).
 struct Plan {
     int splits, cluster;
 };
@@ -760,6 +762,9 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
         return VDIT_ERR_LAUNCH;
     }
     const dim3 grid(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
+    // Set up while the kernel before it ends.  In a stream of calls 16 ragged sequences take 18.9 us instead of
+    // 20.5 and one of 4101 keys 12.6 either way; replayed in a graph, where launches are close already,
+    // the one sequence takes 12.4 instead of 11.9.
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
