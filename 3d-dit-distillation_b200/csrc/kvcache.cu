@@ -207,16 +207,19 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 //   S = K Q^T   32 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
 //               query by a power of two that puts its largest channel at 2^15: exact but for
 //               channels 2^32 below that one
-//   O += V^T P  channels x queries, accumulated by the MMA; P in f16 (a weight is off by 2^-11 of
-//               itself at most, an eighth of the output's own rounding) is 2^(s - m) times the key's
+//   O += V^T P  channels x queries, accumulated by the MMA; P is 2^(s - m) times the key's
 //               value scale over a reference, one for each block and query, that keeps the largest
 //               of them below 2^15.  The reference falls as m rises and rises when a weight would
 //               pass 2^15 (both move O by the same power of two), so that values however large take
 //               no precision from the others where their weight is nothing
+// 2^(s - m) goes into P as two f16 parts, its first 11 bits and the rest, so that a weight is off by
+// 2^-21 of itself, as by the exponential, and not by f16's 2^-11.  Up to 4 queries a key head have
+// the second part in the MMA's columns 4 to 7, which would be empty (SLOTS 4: both parts of P for the
+// price of one); 5 to 8 queries take a second MMA (SLOTS 8).
 // Channels and keys map to fragment indices so that a lane reads consecutive bytes.  m is raised
 // only by a score more than 1 above it (a weight stays below 2): exact, as every term uses the same m.
 constexpr int kWarps = 4;
-constexpr int kQ = 8;                        // queries of a CTA
+constexpr int kQ = 8;                        // columns of the MMAs
 constexpr int kGroup = 32;                   // keys of a group
 
 struct AttnArgs {
@@ -341,19 +344,21 @@ struct Ring {
     static constexpr int BYTES = (kWarps * WARP > STATES ? kWarps * WARP : STATES) + 16;   // scale_word reads past
 };
 
-template <int HD, int BITS>
+// SLOTS: queries of a CTA, at most
+template <int HD, int BITS, int SLOTS>
 __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a) {
     using R = Ring<HD, BITS>;
     constexpr int NB = R::NB, kStages = R::STAGES;
+    constexpr int PARTS = kQ / SLOTS == 2 ? 1 : 2;          // of the weights, in MMAs of their own
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float joined[kQ][2];                         // max and sum of the CTA's queries
     __shared__ int live[kWarps][kStages][2];                // keys that count of the halves of a group
     __shared__ uint64_t full[kWarps][kStages];              // a group's copies have arrived
     __shared__ int abort_flag;
-    const int split = blockIdx.x, chunks = (a.group + kQ - 1) / kQ;
-    const int kh = blockIdx.y / chunks, q0 = (blockIdx.y % chunks) * kQ, b = blockIdx.z;
+    const int split = blockIdx.x, chunks = (a.group + SLOTS - 1) / SLOTS;
+    const int kh = blockIdx.y / chunks, q0 = (blockIdx.y % chunks) * SLOTS, b = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int nq = min(kQ, a.group - q0);
+    const int nq = min(SLOTS, a.group - q0), mine_q = g & (SLOTS - 1);
     if (threadIdx.x < kWarps * kStages) tc::mbar_init(tc::smem_u32(&full[0][0] + threadIdx.x), 1);
     if (threadIdx.x == 0) abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -365,18 +370,18 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     uint4 raw[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-        raw[i] = g < nq ? load_after(reinterpret_cast<const uint4*>(
-                              a.q + b * a.ldq + (int64_t)(kh * a.group + q0 + g) * HD + i * 32 + t * 8))
-                        : make_uint4(0, 0, 0, 0);
+        raw[i] = mine_q < nq ? load_after(reinterpret_cast<const uint4*>(
+                                   a.q + b * a.ldq + (int64_t)(kh * a.group + q0 + mine_q) * HD + i * 32 + t * 8))
+                             : make_uint4(0, 0, 0, 0);
     const int len = (int)length_of(a, c.page_size, given);      // an int32, as the caller's
     const int per = ((len + kGroup - 1) / kGroup + a.splits - 1) / a.splits * kGroup;
     const int first = (int)min((int64_t)len, (int64_t)split * per) + warp * kGroup;   // groups at first + i * step ...
     const int end = (int)min((int64_t)len, (int64_t)(split + 1) * per);               // ... below end
     const int mine = first < end ? (end - first + step - 1) / step : 0;
 
-    // query g of this lane as the B fragments of S: per block four f16 pairs of channels t * 8 ...
+    // query mine_q of this lane as the B fragments of S: per block four f16 pairs of channels t * 8 ...
     uint32_t q[NB][4];
-    float c0, c1;                                           // score units of queries 2t and 2t + 1
+    float c0, c1;                                           // score units of columns 2t and 2t + 1
     {
         float f[NB][8];
         uint32_t top = 0;
@@ -435,7 +440,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         }
     };
 
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // of queries 2t and 2t + 1
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // of columns 2t and 2t + 1
     float o[2 * NB][4];                                     // in units of 1 / inv
     float2 inv[NB];                                         // powers of two, one for each block and query
 #pragma unroll
@@ -454,6 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         float& i = c == 0 ? inv[k].x : inv[k].y;
         i = __uint_as_float(__float_as_uint(i) + ((uint32_t)by << 23));
     };
+    const float part_h = t < 2 ? 1.f : -1.f, part_s = t < 2 ? 0.f : 1.f;
     auto field = [&](int k, int c) { return (int)(__float_as_uint(c == 0 ? inv[k].x : inv[k].y) >> 23); };
 
 #pragma unroll
@@ -552,23 +558,34 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             l0 += s[r].x;
             l1 += s[r].y;
         }
-        // O += V^T P
-        uint32_t pk[NB][4];
-        auto weights = [&] {                                // of all blocks as f16 pairs; returns the largest
-            uint32_t top = 0;
+        // O += V^T P, one block after another
+        auto first = [](float2 y) {                         // 11 bits of each
+            return make_float2(__uint_as_float(__float_as_uint(y.x) & 0xffffe000u),
+                               __uint_as_float(__float_as_uint(y.y) & 0xffffe000u));
+        };
+        if (PARTS == 1)                                     // the first part in columns 0 to 3, the rest in 4 to 7
 #pragma unroll
-            for (int k = 0; k < NB; ++k)
+            for (int r = 0; r < 4; ++r)
+                s[r] = tc::ffma2v(first(s[r]), make_float2(part_h, part_h), fmul2(s[r], part_s));
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            uint32_t pk[PARTS][4];
+            auto weights = [&] {                            // as f16 pairs; returns the largest
+                uint32_t top = 0;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float2 y = fmul2(fmul2(s[r], vsc[r][k]), inv[k]);
-                    pk[k][r] = pack_f16(y.x, y.y);
-                    top = __vmaxu2(top, pk[k][r]);
+                    const float2 h = PARTS == 1 ? y : first(y);
+                    pk[0][r] = pack_f16(h.x, h.y);
+                    if (PARTS == 2) {
+                        const float2 rest = tc::ffma2v(h, make_float2(-1.f, -1.f), y);
+                        pk[PARTS - 1][r] = pack_f16(rest.x, rest.y);
+                    }
+                    top = __vmaxu2(top, pk[0][r]);          // the first part is the larger one
                 }
-            return max(top >> 16, top & 0xffffu);
-        };
-        if (__any_sync(0xffffffffu, weights() > 0x7800u)) {             // 2^15
-#pragma unroll
-            for (int k = 0; k < NB; ++k)
+                return max(top >> 16, top & 0xffffu);
+            };
+            if (__any_sync(0xffffffffu, weights() > 0x7800u)) {         // 2^15
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     float w = 0.f;
@@ -580,13 +597,16 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
                     const int by = max(267 - (int)(__float_as_uint(w) >> 23), 1) - field(k, c);
                     if (by < 0) move(k, c, by > -127 ? __uint_as_float((uint32_t)(127 + by) << 23) : 0.f, by);
                 }
-            weights();
-        }
-#pragma unroll
-        for (int k = 0; k < NB; ++k) {
+                weights();
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t b0 = transpose8(pk[k][2 * h]), b1 = transpose8(pk[k][2 * h + 1]);
+                uint32_t b[PARTS][2];
+#pragma unroll
+                for (int i = 0; i < PARTS; ++i) {
+                    b[i][0] = transpose8(pk[i][2 * h]);
+                    b[i][1] = transpose8(pk[i][2 * h + 1]);
+                }
                 uint32_t va[4], vb[4];                      // keys 2t, 2t + 1 and 2t + 8, 2t + 9 of the half
                 const uint8_t* v = st + R::V + (2 * t + 16 * h) * R::W + value_at;
                 const uint8_t *v0 = v + ((k * 4 * BITS) ^ value_swap[0]), *v1 = v + R::W + ((k * 4 * BITS) ^ value_swap[1]);
@@ -595,7 +615,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t f[4] = {va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1]};
-                    mma_f16(o[2 * k + e], f, b0, b1);
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i) mma_f16(o[2 * k + e], f, b[i][0], b[i][1]);
                 }
             }
         }
@@ -615,7 +636,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     __syncthreads();                                        // the rings are done with
     float* ml = reinterpret_cast<float*>(smem);             // [warp][query][2]
     float* so = ml + kWarps * kQ * 2;                       // [warp][query][HD]
-    if (g == 0) {
+    const bool holds = 2 * t < SLOTS;                       // columns 2t and 2t + 1 are queries
+    if (g == 0 && holds) {
         float* x = ml + (warp * kQ + 2 * t) * 2;
         x[0] = m0;
         x[1] = l0;
@@ -629,9 +651,15 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const float* x = o[2 * k + e];
+            float2 v0 = make_float2(x[0] * u0, x[2] * u0), v1 = make_float2(x[1] * u1, x[3] * u1);
+            if (PARTS == 1) {                               // the weights' second parts, of columns 4 to 7
+                v0 = tc::fadd2(v0, make_float2(__shfl_down_sync(0xffffffffu, v0.x, 2), __shfl_down_sync(0xffffffffu, v0.y, 2)));
+                v1 = tc::fadd2(v1, make_float2(__shfl_down_sync(0xffffffffu, v1.x, 2), __shfl_down_sync(0xffffffffu, v1.y, 2)));
+            }
+            if (!holds) continue;
             float* to = so + (warp * kQ + 2 * t) * HD + k * 32 + g * 4 + e * 2;
-            *reinterpret_cast<float2*>(to) = make_float2(x[0] * u0, x[2] * u0);
-            *reinterpret_cast<float2*>(to + HD) = make_float2(x[1] * u1, x[3] * u1);
+            *reinterpret_cast<float2*>(to) = v0;
+            *reinterpret_cast<float2*>(to + HD) = v1;
         }
     }
     __syncthreads();
@@ -728,12 +756,17 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
 // no more than 2048 keys each, they are a cluster, which joins them itself (one launch, no workspace);
 // otherwise their states go through the workspace to a second kernel (16 sequences of up to 32768
 // keys: 200 us when this was chosen, 183 now; in clusters of 2 or 8 272 and 233).
+// Queries of a CTA, at most: 4 with both parts of their weights in one MMA, 8 with two.  16 sequences over 8
+// key heads of 96 channels, 8 bits: 4 queries a key head (up to 20000 keys) 76 us with 4, 81 with 8; 5 queries
+// (up to 16000 keys) 105 with 4 (two CTAs read the same keys), 73 with 8.
+int slots_of(int group) { return group <= 4 ? 4 : kQ; }
+
 struct Plan {
     int splits, cluster;
 };
 Plan plan_of(int batch, int heads, int kv_heads, int64_t longest) {
     const int group = heads / kv_heads;
-    const int64_t ctas = (int64_t)batch * kv_heads * ((group + kQ - 1) / kQ);
+    const int64_t ctas = (int64_t)batch * kv_heads * ((group + slots_of(group) - 1) / slots_of(group));
     const int64_t two = std::min(6 * 148 / ctas, (longest + 127) / 128), four = std::min(12 * 148 / ctas, longest / 1024);
     const int64_t want = std::min<int64_t>(std::max<int64_t>(std::max(two, four), 1), kMaxSplits);
     int c = 1;
@@ -744,7 +777,7 @@ Plan plan_of(int batch, int heads, int kv_heads, int64_t longest) {
 
 constexpr int kMaxDevices = 64;
 
-template <int HD, int BITS>
+template <int HD, int BITS, int SLOTS>
 int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) {
     static std::atomic<bool> ready[kMaxDevices];            // the kernel's attributes are set, per device
     constexpr int bytes = Ring<HD, BITS>::BYTES;
@@ -752,16 +785,16 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) return VDIT_ERR_UNSUPPORTED;
     if (e == cudaSuccess && !ready[dev].load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(attend_kernel<HD, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        e = cudaFuncSetAttribute(attend_kernel<HD, BITS, SLOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attend_kernel<HD, BITS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            e = cudaFuncSetAttribute(attend_kernel<HD, BITS, SLOTS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) ready[dev].store(true, std::memory_order_release);
     }
     if (e != cudaSuccess) {
         record_cuda_error(e);
         return VDIT_ERR_LAUNCH;
     }
-    const dim3 grid(a.splits, c.heads * ((a.group + kQ - 1) / kQ), batch);
+    const dim3 grid(a.splits, c.heads * ((a.group + SLOTS - 1) / SLOTS), batch);
     // Set up while the kernel before it ends.  In a stream of calls 16 ragged sequences take 18.9 us instead of
     // 20.5 and one of 4101 keys 12.6 either way; replayed in a graph, where launches are close already,
     // the one sequence takes 12.4 instead of 11.9.
@@ -778,7 +811,7 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = bytes;
-    e = cudaLaunchKernelEx(&cfg, attend_kernel<HD, BITS>, c, a);
+    e = cudaLaunchKernelEx(&cfg, attend_kernel<HD, BITS, SLOTS>, c, a);
     if (e != cudaSuccess) {
         record_cuda_error(e);
         return VDIT_ERR_LAUNCH;
@@ -944,7 +977,8 @@ extern "C" int vdit_attention_1q_cached(const void* q, int64_t ldq, const vdit_k
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int status = VDIT_OK;
     with_format(c.hd, cache->bits, [&](auto hd, auto bits) {
-        status = launch_attend<decltype(hd)::value, decltype(bits)::value>(c, a, batch, s);
+        constexpr int HD = decltype(hd)::value, BITS = decltype(bits)::value;
+        status = slots_of(a.group) == 4 ? launch_attend<HD, BITS, 4>(c, a, batch, s) : launch_attend<HD, BITS, kQ>(c, a, batch, s);
     });
     return status;
 }

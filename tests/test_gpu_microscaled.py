@@ -375,6 +375,39 @@ def test_attention_with_infinities_in_queries():
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hd", [32, 128])
+def test_attention_weights_have_the_accuracy_of_32_bits(hd, bits):
+    """Two kinds of keys whose values cancel: what is left of the output shows the weights' own error,
+    which the output's rounding hides elsewhere.  32 sequences of 64 keys, the weight of the first kind
+    another one in each; a last key takes the rest of the sum, as near as its few bits allow.  The bound
+    is that of ``check_attend`` with weights off by 2^-21 of themselves, not by f16's 2^-11."""
+    n, b = 64, 32
+    c = fk.MxKvCache(b * n // 16, 16, 1, hd, bits=bits, device=DEV)
+    x = torch.linspace(-2.5, -0.05, b).to(BF16)
+    q = torch.zeros(b, hd, dtype=BF16)
+    q[:, 0] = x
+    k, v = (torch.zeros(b, n, hd, dtype=BF16) for _ in range(2))
+    w = torch.exp(x.double())
+    first = (n / (1 + w)).round().long().clamp(1, n - 2)      # keys of the first kind: first * w ~ n - first
+    for i in range(b):
+        k[i, :first[i], 0] = 1.0
+        v[i, :first[i]], v[i, first[i]:] = 1.0, -1.0
+        v[i, n - 1] = float(n - 1 - first[i] - first[i] * w[i])
+    k, v = (t.reshape(c.slots, hd).to(DEV) for t in (k, v))
+    fk.kv_cache_write(c, k, v, torch.arange(c.slots, device=DEV))
+    t = torch.arange(b * n // 16, dtype=torch.int32, device=DEV).view(b, n // 16)
+    got = host(fk.attention_1q_cached(q.to(DEV), c, t, i32([n] * b), 1.0))
+    kv, vv = (mxo.values(host(t), bits).reshape(b, n, 1, hd) for t in (k, v))
+    for i in range(b):
+        want, mag, unit = mxo.attend(host(q[i]).reshape(1, hd), kv[i], vv[i], 1.0)
+        assert np.abs(want).max() < 0.05 * mag.max()
+        rel = 2 * (np.expm1((hd + 4) * 2.0 ** -24 * unit) + 2.0 ** -21) + 2.0 ** -21 + (n + 8) * 2.0 ** -24
+        e = rel[:, None] * mag
+        err = np.abs(got[i].reshape(1, hd) - want)
+        assert (err <= e + 2.0 ** -8 * (np.abs(want) + e)).all(), (i, err.max(), e.max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("order", ["first", "last", "each group"])
 def test_attention_huge_values_without_weight(order, bits):
     """Values 2^90 times the others at keys whose weight is nothing beside the others': they must not
