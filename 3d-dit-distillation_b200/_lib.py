@@ -70,6 +70,8 @@ SIGNATURES = {
     "vdit_linear": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i32, _c_i32, _vp]),
     "vdit_linear_qkv_rope3d": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _vp,
                                               _vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _vp]),
+    "vdit_wait_limit_ms": (ctypes.c_int, []),
+    "vdit_wait_check": (ctypes.c_int, [_vp]),
     "vdit_mxfp4_scale_bytes": (_c_sz, [_c_i64, _c_i32]),
     "vdit_mxfp4_quantize": (ctypes.c_int, [_vp, _c_i32, _c_i64, _c_i64, _c_i32, _vp, _vp, _vp]),
     "vdit_mxfp4_dequantize": (ctypes.c_int, [_vp, _vp, _c_i64, _c_i32, _vp, _c_i32, _c_i64, _vp]),

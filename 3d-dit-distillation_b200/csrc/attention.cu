@@ -484,6 +484,7 @@ int rowops_error_word(int clear);       // error word of the staged row kernels 
 int gemm_error_word(int clear);         // error word of the tcgen05 GEMM (gemm.cu)
 int unpatch_error_word(int clear);      // error word of the unpatchify projection (unpatchify.cu)
 int patchify_error_word(int clear);     // error word of the tensor-core patchify (patchify.cu)
+int wait_check_error_word(int clear);   // error word of the check of the waits' limit (runtime.cu)
 }
 
 extern "C" int vdit_device_error(int clear) {
@@ -506,7 +507,9 @@ extern "C" int vdit_device_error(int clear) {
     if (u < 0) return u;
     const int t = vdit::patchify_error_word(clear);
     if (t < 0) return t;
-    for (int w : {v, d, p, r, g, u, t})
+    const int c = vdit::wait_check_error_word(clear);
+    if (c < 0) return c;
+    for (int w : {v, d, p, r, g, u, t, c})
         if (w != 0) return w;
     return 0;
 }

@@ -5,8 +5,39 @@
 #include <cstdio>
 
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace vdit {
+
+__device__ int g_wait_check_error = 0;
+
+namespace {
+
+constexpr int kErrWaitCheck = 0x5754;   // "WT": the wait of vdit_wait_check ran out, as it should
+
+// one warp waits for an arrival that nothing makes
+__global__ void wait_check_kernel() {
+    __shared__ uint64_t bar;
+    __shared__ int abort_flag;
+    if (threadIdx.x == 0) {
+        tc::mbar_init(tc::smem_u32(&bar), 1);
+        abort_flag = 0;
+    }
+    __syncthreads();
+    tc::mbar_wait(tc::smem_u32(&bar), 0, &abort_flag, &g_wait_check_error, kErrWaitCheck);
+}
+
+}  // namespace
+
+int wait_check_error_word(int clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_wait_check_error, sizeof(int)) != cudaSuccess) return VDIT_ERR_LAUNCH;
+    if (clear) {
+        int z = 0;
+        if (cudaMemcpyToSymbol(g_wait_check_error, &z, sizeof(int)) != cudaSuccess) return VDIT_ERR_LAUNCH;
+    }
+    return v;
+}
 
 static std::atomic<long long> g_launches{0};
 
@@ -36,6 +67,14 @@ extern "C" const char* vdit_error_string(int code) {
         case VDIT_ERR_TOO_LARGE: return "size exceeds the fixed scratch of the no-alloc entry point";
         default: return "unknown error";
     }
+}
+
+extern "C" int vdit_wait_limit_ms(void) { return (int)(vdit::tc::kWaitLimitNs / 1000000u); }
+
+extern "C" int vdit_wait_check(vdit_stream_t stream) {
+    vdit::wait_check_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>();
+    vdit::count_launches(1);
+    return vdit::check_launch();
 }
 
 extern "C" long long vdit_launch_count(void) { return vdit::g_launches.load(std::memory_order_relaxed); }

@@ -51,6 +51,14 @@ long long vdit_launch_count(void);
  * index out of range seen by a kernel).  Synchronizes the device; clear!=0
  * resets the word.  Returns 0 when no error was recorded. */
 int vdit_device_error(int clear);
+/* Every wait of a kernel for a copy, a matrix product or another warp gives up after this many
+ * milliseconds: the kernel records its code in the device error word and ends.  (Barriers of a
+ * cluster, the allocation of tensor memory and the completion of a kernel's own stores are waits of
+ * the hardware's and have no such limit.) */
+int vdit_wait_limit_ms(void);
+/* Shows that limit at work: launches one warp that waits for an arrival that nothing makes.  The
+ * launch ends after vdit_wait_limit_ms(), and the device error word then holds 0x5754. */
+int vdit_wait_check(vdit_stream_t stream);
 
 /* ------------------------------------------------------------------ geometry */
 /* Workspace (bytes) for vdit_lex_perm / vdit_hilbert4_orders on n voxels. */
