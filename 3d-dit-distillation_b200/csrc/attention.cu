@@ -67,6 +67,7 @@ struct SegInfo {
 //   pfull(b)   P(j) in TMEM (128 arrivals), phase j / 2
 //   pvdone(b)  every MMA up to PV(j) complete, phase j / 2 (awaited only before a rescale)
 //   odone      the last PV complete
+//   drained    after an abort: every MMA issued has ended
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_constant__ CUtensorMap tmK,
                                                               const __grid_constant__ CUtensorMap tmV,
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
 
     const uint32_t b_q = smem_u32(&bars[0]);
     constexpr int KB = 1, VB = KB + 2 * KSTAGES, SB = VB + 2 * VSTAGES;   // barrier index bases
-    static_assert(SB + 3 * NS + 1 <= 24, "barrier slots");
+    static_assert(SB + 3 * NS + 2 <= 24, "barrier slots");
     auto b_kfull = [&](int s) { return smem_u32(&bars[KB + s]); };
     auto b_kempty = [&](int s) { return smem_u32(&bars[KB + KSTAGES + s]); };
     auto b_vfull = [&](int s) { return smem_u32(&bars[VB + s]); };
@@ -102,6 +103,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
     auto b_pfull = [&](int b) { return smem_u32(&bars[SB + NS + b]); };
     auto b_pvdone = [&](int b) { return smem_u32(&bars[SB + 2 * NS + b]); };
     const uint32_t b_odone = smem_u32(&bars[SB + 3 * NS]);
+    const uint32_t b_drained = smem_u32(&bars[SB + 3 * NS + 1]);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = blockIdx.y;
@@ -138,6 +140,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
             mbar_init(b_pvdone(b), 1);
         }
         mbar_init(b_odone, 1);
+        mbar_init(b_drained, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmK)) : "memory");
@@ -151,6 +154,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    int fills = 0;                                          // producers: loads issued into their ring
 
     if (warp == 0 || warp == 6) {
         // ------------------------------------------------------------ TMA producers (K: warp 0, V: warp 6)
@@ -166,6 +170,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
                 if (j >= nst && !mbar_wait(empty, ((j - nst) / nst) & 1, abort_flag, &g_device_error, kErrTimeout))
                     break;
                 mbar_expect_tx(full, TILE);
+                ++fills;
                 for (int c = 0; c < NCH; ++c)
                     tma_load_3d(smem_u32(ring + st * TILE + c * CHUNK), map, c * 32, head, k_begin + j * BN, full);
             }
@@ -367,6 +372,20 @@ __global__ void __launch_bounds__(THREADS, 1) attention_kernel(const __grid_cons
 
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {
+        // a wait ran out: the loads and MMAs still in flight end before the CTA does
+        if (warp == 1) {
+            volatile int gave_up = 0;
+            tc_commit_elect(b_drained);
+            mbar_wait(b_drained, 0, &gave_up, &g_device_error, kErrTimeout);
+            __syncwarp();
+        } else if (lane == 0 && warp == 0) {
+            drain_loads(0, fills, KSTAGES, b_kfull, &g_device_error, kErrTimeout);
+        } else if (lane == 0 && warp == 6) {
+            drain_loads(0, fills, VSTAGES, b_vfull, &g_device_error, kErrTimeout);
+        }
+        __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));

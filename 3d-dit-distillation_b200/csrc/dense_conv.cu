@@ -39,7 +39,7 @@ struct __align__(1024) Smem {
     uint8_t a[S][MT][BM * 128];
     uint8_t b[S][BN * 128];
     int32_t idx[ROWS * 27];
-    uint64_t full_a[S], full_b[S], empty[S], acc_full;
+    uint64_t full_a[S], full_b[S], empty[S], acc_full, drained;   // drained: after an abort, every MMA issued has ended
     uint32_t tmem_slot;
     int abort_flag;
     unsigned tapmask;
@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(THREADS, 1) dense_conv27_kernel(const __grid_c
             mbar_init(smem_u32(&sm.empty[s]), 1);
         }
         mbar_init(smem_u32(&sm.acc_full), 1);
+        mbar_init(smem_u32(&sm.drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW)) : "memory");
     }
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(THREADS, 1) dense_conv27_kernel(const __grid_c
     const unsigned mask = sm.tapmask;
     const int nkc = cin / BK;
     const int n_iter = __popc(mask) * nkc;
+    int fills = 0;                                          // weight tiles: loads issued
 
     if (warp < GATHER_WARPS) {
         // ------------------------------------------------------------ A gather
@@ -179,6 +181,7 @@ __global__ void __launch_bounds__(THREADS, 1) dense_conv27_kernel(const __grid_c
                 if (i >= S && !mbar_wait(smem_u32(&sm.empty[s]), ((i / S) - 1) & 1, abort_flag, &g_dense_error, kErr))
                     break;
                 mbar_expect_tx(smem_u32(&sm.full_b[s]), BN * 128);
+                ++fills;
                 tma_load_2d(smem_u32(sm.b[s]), &tmW, tw.kc * BK, tw.tap * cout + co0, smem_u32(&sm.full_b[s]));
             }
         }
@@ -216,6 +219,18 @@ __global__ void __launch_bounds__(THREADS, 1) dense_conv27_kernel(const __grid_c
 
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {
+        // a wait ran out: the loads and MMAs still in flight end before the CTA does
+        if (warp == GATHER_WARPS + 1) {
+            volatile int gave_up = 0;
+            tc_commit_elect(smem_u32(&sm.drained));
+            mbar_wait(smem_u32(&sm.drained), 0, &gave_up, &g_dense_error, kErr);
+            __syncwarp();
+        } else if (warp == GATHER_WARPS && lane == 0) {
+            drain_loads(0, fills, S, [&](int s) { return smem_u32(&sm.full_b[s]); }, &g_dense_error, kErr);
+        }
+        __syncthreads();
+    }
     if (warp == GATHER_WARPS + 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));

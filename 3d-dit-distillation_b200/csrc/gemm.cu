@@ -62,8 +62,10 @@ struct __align__(1024) Smem {
     uint8_t b[NST][BN / 2 * 128];    // this CTA's half of the weight tile
     uint8_t x[XBYTES];
     uint64_t full[NST], empty[NST], acc_full[2], acc_empty[2];
+    uint64_t drained;                // after an abort: every MMA issued has ended
     uint32_t tmem_slot;
     int abort_flag;
+    int peer_fills;                  // after an abort: the loads that the other CTA of the pair issued
 };
 
 struct EpiArgs {
@@ -137,6 +139,7 @@ __global__ void __launch_bounds__(threads_of<EPI>(), 1) gemm_kernel(const __grid
             mbar_init(smem_u32(&sm.acc_full[b]), 1);
             mbar_init(smem_u32(&sm.acc_empty[b]), 2 * epi_warps<EPI>());
         }
+        mbar_init(smem_u32(&sm.drained), 1);
         sm.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmA)) : "memory");
@@ -160,11 +163,12 @@ __global__ void __launch_bounds__(threads_of<EPI>(), 1) gemm_kernel(const __grid
     cluster_sync();    // the peer's barriers are initialised before anyone signals them
     tc_fence_after();
     const uint32_t tmem = sm.tmem_slot;
+    int fills = 0;                   // producer: loads issued into the ring
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (both CTAs)
         if (lane == 0) {
-            int it = 0;
+            int& it = fills;
             bool ok = true;
             for (int t = pair; ok && t < ntiles; t += npairs) {
                 int tm, tn;
@@ -359,7 +363,26 @@ __global__ void __launch_bounds__(threads_of<EPI>(), 1) gemm_kernel(const __grid
 
     tc_fence_before();
     __syncthreads();
+    // an abort is the pair's: the peer need not wait its own limit out
+    if (threadIdx.x == 0 && *abort_flag) store_cluster(mapa_shared(smem_u32(&sm.abort_flag), rank ^ 1), 1);
+    __syncwarp();
     cluster_sync();    // no CTA leaves while its peer's MMAs or arrivals may still touch it
+    if (*abort_flag) {
+        // a wait ran out: the loads and MMAs still in flight end before either CTA does
+        if (threadIdx.x == 0) store_cluster(mapa_shared(smem_u32(&sm.peer_fills), rank ^ 1), fills);
+        __syncwarp();
+        cluster_sync();
+        if (leader && warp == 1) {
+            volatile int gave_up = 0;
+            tc_commit_pair_elect(smem_u32(&sm.drained), 0x1);
+            mbar_wait(smem_u32(&sm.drained), 0, &gave_up, &g_gemm_error, kErr);
+        } else if (leader && threadIdx.x == 0) {
+            drain_pair_loads(fills, sm.peer_fills, STAGES, kStageBytes, [&](int s) { return smem_u32(&sm.full[s]); },
+                             &g_gemm_error, kErr);
+        }
+        __syncthreads();
+        cluster_sync();
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));

@@ -471,9 +471,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     const int value_swap[2] = {((BITS == 8 ? g >> 2 : 0) ^ swapped_piece<R::CH>(2 * t)) << 4,
                                ((BITS == 8 ? g >> 2 : 0) ^ swapped_piece<R::CH>(2 * t + 1)) << 4};
     int seen = 0;                                           // whether any key of this warp counted
+    int done = 0;                                           // groups worked off
     int cur = 0, next = kStages - 1;                        // the stage of this step and the one its copies go to
     uint32_t phase = 0;                                     // of the stages' barriers
-    for (int i = 0; i < mine; ++i) {
+    for (int i = 0; i < mine; ++i, ++done) {
         __syncwarp();                                       // every lane has read the stage that is filled next
         issue(i + kStages - 1, next);
         if (!__all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&full[warp][cur]), phase, &abort_flag, &g_kvcache_error,
@@ -621,6 +622,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
             }
         }
     }
+    // after an abort: the copies still on their way land before the ring becomes the place of the states
+    if (done < mine)
+        tc::drain_loads(done, min(mine, done + kStages), kStages,
+                        [&](int s) { return tc::smem_u32(&full[warp][s]); }, &g_kvcache_error, kErrWait);
     // a warp whose scores were all -inf (a query with infinities) has seen keys, unlike an empty one:
     // alone it makes 0 / 0, not zeros
     if (seen) {

@@ -55,8 +55,10 @@ struct __align__(1024) Smem {
     uint8_t sw[NST][NBLK][2 * kScaleBlock];                 // the scales of the whole weight tile
     float bias[EPI_WARPS][BN];
     uint64_t full[NST], empty[NST], acc_full[2], acc_empty[2], shared_empty;
+    uint64_t drained;                                       // after an abort: every MMA issued has ended
     uint32_t tmem_slot;
     int abort_flag;
+    int peer_fills;                                         // after an abort: the loads that the pair's other CTA issued
 };
 
 struct Args {
@@ -140,6 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
             mbar_init(smem_u32(&sm.acc_empty[b]), CG * EPI_WARPS);
         }
         mbar_init(smem_u32(&sm.shared_empty), CG * EPI_WARPS);
+        mbar_init(smem_u32(&sm.drained), 1);
         sm.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (const CUtensorMap* map : {&tmA, &tmW, &tmSA, &tmSW, &tmO})
@@ -163,6 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     // all 512 columns are this CTA's, so they start at 0: a constant, as MMA operands from shared
     // memory would pass through vector registers
     constexpr uint32_t tmem = 0;
+    int fills = 0;                                          // producer: loads issued into the ring
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (every CTA)
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
             // a is written, when launched beside its writer.  That one lets this kernel start only after
             // its own wait, so all older kernels are complete: the epilogue reads the bias without a wait.
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            int it = 0;
+            int& it = fills;
             bool ok = true;
             for (int t = unit; ok && t < ntiles; t += nunits) {
                 int tm, tn;
@@ -321,7 +325,32 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
 
     tc_fence_before();
     __syncthreads();
-    if (CG == 2) cluster_sync();     // no CTA leaves while its peer's MMAs or arrivals may still touch it
+    if (CG == 2) {
+        // an abort is the pair's: the peer need not wait its own limit out
+        if (threadIdx.x == 0 && *abort_flag) store_cluster(mapa_shared(smem_u32(&sm.abort_flag), rank ^ 1), 1);
+        __syncwarp();
+        cluster_sync();              // no CTA leaves while its peer's MMAs or arrivals may still touch it
+    }
+    if (*abort_flag) {
+        // a wait ran out: the loads and MMAs still in flight end before any CTA of them does
+        if (CG == 2) {
+            if (threadIdx.x == 0) store_cluster(mapa_shared(smem_u32(&sm.peer_fills), rank ^ 1), fills);
+            __syncwarp();
+            cluster_sync();
+        }
+        auto full = [&](int s) { return smem_u32(&sm.full[s]); };
+        if (rank == 0 && warp == 1) {
+            volatile int gave_up = 0;
+            if constexpr (CG == 1) tc_commit_elect(smem_u32(&sm.drained));
+            else tc_commit_pair_elect(smem_u32(&sm.drained), 0x1);
+            mbar_wait(smem_u32(&sm.drained), 0, &gave_up, &g_mxlinear_error, kErr);
+        } else if (rank == 0 && threadIdx.x == 0) {
+            if (CG == 1) drain_loads(0, fills, NST, full, &g_mxlinear_error, kErr);
+            else drain_pair_loads(fills, sm.peer_fills, NST, kStageBytes / 2, full, &g_mxlinear_error, kErr);
+        }
+        __syncthreads();
+        if (CG == 2) cluster_sync();
+    }
     if (warp == 1) {
         tc_fence_after();
         if constexpr (CG == 1)

@@ -84,6 +84,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// The end of an aborted CTA.  Waits (bounded) for the last fills of a ring of loads: fill j went to stage
+// j % stages and completes phase j / stages of full(stage).  Called by one thread before the CTA leaves or
+// uses the ring for something else, so that no copy lands in memory that is no longer the ring's.
+template <typename F>
+__device__ __forceinline__ void drain_loads(int first, int issued, int stages, F&& full, int* err, int code) {
+    volatile int gave_up = 0;
+    for (int j = max(first, issued - stages); j < issued; ++j)
+        if (!mbar_wait(full(j % stages), (uint32_t)(j / stages) & 1, &gave_up, err, code)) return;
+}
+
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -315,6 +325,29 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t cta) {
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// a word of another CTA's shared memory (shared::cluster address)
+__device__ __forceinline__ void store_cluster(uint32_t cluster_addr, int v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
+// The end of a pair of which either CTA aborted; the even CTA's part (the odd one waits at the cluster
+// barrier behind it).  Every load of the pair counts on the even CTA's barriers, full(stage), which it
+// armed for its own `mine` fills with both CTAs' bytes.  Where only one of the two issued a fill, the
+// odd CTA's bytes are made up for: counted as there, or armed for alone once the stage's fill before is
+// complete.
+template <typename F>
+__device__ __forceinline__ void drain_pair_loads(int mine, int odd, int stages, uint32_t odd_bytes, F&& full, int* err,
+                                                 int code) {
+    volatile int gave_up = 0;
+    for (int j = max(0, mine - stages); j < max(mine, odd); ++j) {
+        const uint32_t bar = full(j % stages);
+        if (j >= mine) mbar_expect_tx(bar, odd_bytes);
+        else if (j >= odd)
+            asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(odd_bytes) : "memory");
+        if (!mbar_wait(bar, (uint32_t)(j / stages) & 1, &gave_up, err, code)) return;
+    }
 }
 
 // arrive on an mbarrier of another CTA of the cluster (shared::cluster address)
