@@ -188,6 +188,10 @@ __global__ void __launch_bounds__(threads_of<EPI>(), 1) gemm_kernel(const __grid
                     tma_load_2d_pair(smem_u32(sm.b[s]), &tmW, kb * BK, wrow, bar);
                 }
             }
+            // every commit on this CTA's stages has arrived before it leaves: the tensor core delivers them to
+            // both CTAs by itself, which the cluster barrier at the end does not wait for
+            for (int j = max(0, it - STAGES); ok && j < it; ++j)
+                ok = mbar_wait(smem_u32(&sm.empty[j % STAGES]), (j / STAGES) & 1, abort_flag, &g_gemm_error, kErr);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (even CTA)

@@ -195,6 +195,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
                     load_box<CG>(smem_u32(sm.w[s]), &tmW, kb * 128, tn * BN + (int)rank * BNC, bar);
                 }
             }
+            // every commit on this CTA's stages has arrived before it leaves: the tensor core delivers them to
+            // both CTAs of a pair by itself, which the cluster barrier at the end does not wait for
+            for (int j = max(0, it - NST); ok && j < it; ++j)
+                ok = mbar_wait(smem_u32(&sm.empty[j % NST]), (j / NST) & 1, abort_flag, &g_mxlinear_error, kErr);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (even CTA)

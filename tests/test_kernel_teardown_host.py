@@ -30,3 +30,10 @@ def test_tensor_memory_is_freed_after_the_last_product(name):
     text = FILES[name]
     assert text.index("drained") < text.index("tcgen05.dealloc")
     assert re.search(r"tc_commit_(pair_)?elect\((smem_u32\(&sm\.drained\)|b_drained)", text)
+
+
+@pytest.mark.parametrize("name", ["gemm.cu", "mxlinear.cu"])
+def test_a_cta_of_a_pair_leaves_after_every_commit_on_its_stages(name):
+    """The tensor core delivers a commit to both CTAs by itself; each waits for the last one of every stage."""
+    assert re.search(r"for \(int j = max\(0, it - (NST|STAGES)\); ok && j < it; \+\+j\)\s*"
+                     r"ok = mbar_wait\(smem_u32\(&sm\.empty\[", FILES[name])
