@@ -18,6 +18,7 @@ host's cores instead.
 from __future__ import annotations
 
 import argparse
+import faulthandler
 import json
 import math
 import os
@@ -103,6 +104,34 @@ class ClockSampler:
                     reasons.add(n)
         return {"sm_mhz": statistics.median(sm) if sm else None, "sm_max_mhz": mx, "reasons": sorted(reasons),
                 "samples": len(sm)}
+
+
+class Phases:
+    """Says on stderr what begins, and ends the process (exit code 1, every thread's stack on stderr)
+    when one phase lasts longer than ``limit_s``: a kernel that does not end would otherwise hold the GPU
+    for as long as the caller allows, and leave no word of where.  The phase before is checked first:
+    a kernel wait that ran out is named by its code."""
+
+    def __init__(self, limit_s: float = 300.0, rank: int = 0, error_word=None):
+        self.limit_s, self.rank, self.error_word, self.name, self.start = limit_s, rank, error_word, None, time.time()
+
+    def check(self):
+        code = self.error_word() if self.error_word is not None else 0
+        if code:
+            raise SystemExit(f"bench: device error word {code:#x} ({code.to_bytes(4, 'big').strip(bytes(1))!r}) after "
+                             f"phase '{self.name}'")
+
+    def __call__(self, name: str):
+        if self.name is not None:
+            self.check()
+        self.name = name
+        if self.rank == 0:
+            print(f"[bench {time.time() - self.start:7.1f} s] {name}", file=sys.stderr, flush=True)
+        faulthandler.dump_traceback_later(self.limit_s, exit=True)
+
+    def done(self):
+        self.check()
+        faulthandler.cancel_dump_traceback_later()
 
 
 def _l2_flush(buf: torch.Tensor):
@@ -649,7 +678,7 @@ def graph_bench(w, reps: int = 5):
 
 
 def c5_bench(rank: int, ws: int, dev, dist, samples: int = 0, steps: int = 1, warmup: int = 1,
-             model=None) -> dict:
+             model=None, phase=lambda name: None) -> dict:
     """The sharded batch: ``samples`` C5 samples (N=32768 ellipsoid-union voxels in 128^3,
     default 16) split round-robin over the ranks, latents gathered to rank 0 over NCCL.
     One step processes the whole batch once (strong scaling: the batch is fixed, the
@@ -665,9 +694,11 @@ def c5_bench(rank: int, ws: int, dev, dist, samples: int = 0, steps: int = 1, wa
     samples = samples or w.samples
     if samples % ws:
         raise SystemExit(f"{samples} C5 samples do not split evenly over {ws} ranks")
+    phase("C5 weights")
     model = LatDitModel(w.arch, model.state) if model is not None else LatDitModel.random(w.arch, seed=0, device=dev)
     solver = SolverConfig(num_inference_steps=4, n_guided_steps=3, n_unguided_steps=1, guidance_scale=w.guidance)
     runner = Solution(model, solver_config=solver, device=dev).runner
+    phase("C5 inputs")
     inps = [w.inputs(seed=500 + i, device=dev) for i in range(rank, samples, ws)]
     flush = torch.empty(64 * 1024 * 1024, dtype=torch.float32, device=dev)
     s = torch.cuda.current_stream()
@@ -684,8 +715,10 @@ def c5_bench(rank: int, ws: int, dev, dist, samples: int = 0, steps: int = 1, wa
                 e1.record(s)
                 gather_evs.append((e0, e1))
 
+    phase("C5 warm-up")
     for _ in range(warmup):
         step()
+    phase("C5 timed steps")
     evs = [(torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)) for _ in range(steps)]
     launches0 = _lib.launch_count()
     if dist is not None:
@@ -851,6 +884,8 @@ def main():
     dev = torch.device("cuda", local)
     torch.cuda.set_device(dev)
     w = C4()
+    # two seconds a step are six times what one takes
+    phase = Phases(300.0 + 2.0 * (args.steps + args.warmup), rank, _lib.device_error)
     if args.only == "c5":
         r = c5_bench(rank, ws, dev, dist, samples=args.samples, steps=args.steps, warmup=args.warmup)
         if rank == 0:
@@ -901,6 +936,7 @@ def main():
         print(json.dumps({"kernel": "dwconv_planned_kernel (fused SwiGLU)", "ms_per_launch": ms,
                           "gbs": byts / ms / 1e6, "gather_kernel_ms": ms_gather}))
         return
+    phase("model and weights")
     model = LatDitModel.random(w.arch, seed=0, device=dev)
     solver = SolverConfig(num_inference_steps=4, n_guided_steps=3, n_unguided_steps=1, guidance_scale=w.guidance)
     sol = Solution(model, solver_config=solver, device=dev)
@@ -914,6 +950,7 @@ def main():
             vd.gather_latents([lat], rank, ws)
         return lat
 
+    phase("warm-up")
     for _ in range(args.warmup):
         step()
     torch.cuda.synchronize()
@@ -926,6 +963,7 @@ def main():
         return
 
     # ---------------------------------------------------------------- timed region (device time)
+    phase("timed steps")
     s = torch.cuda.current_stream()
     evs = [(torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)) for _ in range(args.steps)]
     launches0 = _lib.launch_count()
@@ -949,6 +987,7 @@ def main():
     launches = (_lib.launch_count() - launches0) // max(args.steps, 1)
     # every kernel class of the forward, in one more sample after the timed steps (not timed
     # as a step): CUDA events around each launch on its stream
+    phase("one sample with every kernel timed")
     kstep: dict = {}
     _l2_flush(flush)
     runner.kernel_timer = kstep
@@ -964,6 +1003,7 @@ def main():
     value = ws * NFE_PER_SAMPLE * w.n / (ms_step / 1e3)
 
     # ---------------------------------------------------------------- per-branch NFE times
+    phase("one NFE of each branch")
     geom = runner._prepare_sample_geometry([inp["vox"]], inp["context"])
     xs = inp["noise"][geom["perm"]].contiguous()
     nfe = {}
@@ -997,6 +1037,7 @@ def main():
     runner.overlap_context = overlap
 
     # ---------------------------------------------------------------- e2e through the plugin API
+    phase("end to end")
     vox_h = inp["vox_host"].pin_memory()
     dino_h = inp["dino_host"].pin_memory()
     cond = LatDitConditioning(dino_features=dino_h, batch_size=1)
@@ -1036,18 +1077,21 @@ def main():
     # in guided steps the conditional and the 1-token NFE run on two streams and share the GPU
     solo = [(a, b) for a, b, _, shared in att_events if not shared]
     solo_ms = statistics.fmean(a.elapsed_time(b) for a, b in solo) if solo else None
+    phase("attention alone")
     flops_alone, att_ms_alone = attention_roofline(w, runner)
     traffic = attention_traffic()
     kernels = kernel_table(kstep, hbm, tflops_sustained, peak_kind, solo=ksolo)
     assert _lib.device_error() == 0, "device error word set during the benchmark"
 
     # ---------------------------------------------------------------- C5 sharded batch (strong scaling)
+    phase("free the C4 model")
     c5 = None
     if not args.no_c5:
         del sol, runner
         torch.cuda.empty_cache()
-        c5 = c5_bench(rank, ws, dev, dist, steps=args.c5_steps, warmup=1, model=model)
+        c5 = c5_bench(rank, ws, dev, dist, steps=args.c5_steps, warmup=1, model=model, phase=phase)
 
+    phase("CPU baseline")
     cpu = None
     if rank == 0 and ws == 1 and not args.no_cpu_baseline:
         threads = os.cpu_count() or 1
@@ -1055,6 +1099,7 @@ def main():
         cpu = {"value": v, "unit": UNIT, "cores": threads, "kind": "port",
                "sample": f"{CPU_SAMPLE} ({dt:.1f} s)"}
 
+    phase.done()
     if rank == 0:
         print(json.dumps({
             "metric": METRIC, "value": value, "unit": UNIT, "n_gpus": ws, "steps": args.steps,
