@@ -206,7 +206,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, const int64_t* 
 // 32-channel block:
 //   S = K Q^T   32 keys x 8 queries, times each key's scale in fp32.  Q is f16 after scaling each
 //               query by a power of two that puts its largest channel at 2^15: exact but for
-//               channels 2^32 below that one
+//               channels 2^32 below that one.  What undoes it (and the softmax's scale) goes into the
+//               key's scale where it makes numbers smaller and behind the sum where it makes them
+//               larger, so that no sum overflows that the score itself does not
 //   O += V^T P  channels x queries, accumulated by the MMA; P is 2^(s - m) times the key's
 //               value scale over a reference, one for each block and query, that keeps the largest
 //               of them below 2^15.  The reference falls as m rises and rises when a weight would
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 
     // query mine_q of this lane as the B fragments of S: per block four f16 pairs of channels t * 8 ...
     uint32_t q[NB][4];
-    float c0, c1;                                           // score units of columns 2t and 2t + 1
+    float2 before, after;                                   // score units of columns 2t and 2t + 1
     {
         float f[NB][8];
         uint32_t top = 0;
@@ -400,8 +402,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         const uint32_t e = top >> 23;
         const uint32_t up = e == 0 || e == 255 ? 127u : min(253u, 269u - e);    // exponent field of the factor
         const float unit = __uint_as_float((254u - up) << 23) * a.scale_log2;
-        c0 = __shfl_sync(0xffffffffu, unit, 8 * t);
-        c1 = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+        const float2 c = make_float2(__shfl_sync(0xffffffffu, unit, 8 * t), __shfl_sync(0xffffffffu, unit, 8 * t + 4));
+        before = make_float2(fabsf(c.x) <= 1.f ? c.x : 1.f, fabsf(c.y) <= 1.f ? c.y : 1.f);
+        after = make_float2(fabsf(c.x) <= 1.f ? 1.f : c.x, fabsf(c.y) <= 1.f ? 1.f : c.y);
         const float fac = __uint_as_float(up << 23);
 #pragma unroll
         for (int i = 0; i < NB; ++i)
@@ -518,14 +521,13 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
                 const uint32_t f0[4] = {ka[0], kb[0], ka[1], kb[1]}, f1[4] = {ka[2], kb[2], ka[3], kb[3]};
                 mma_f16(d, f0, q[k][0], q[k][1]);
                 mma_f16(d, f1, q[k][2], q[k][3]);
-                const float sa = ksc[2 * h][k], sb = ksc[2 * h + 1][k];
-                s[2 * h] = tc::ffma2v(make_float2(d[0], d[1]), make_float2(sa, sa), s[2 * h]);
-                s[2 * h + 1] = tc::ffma2v(make_float2(d[2], d[3]), make_float2(sb, sb), s[2 * h + 1]);
+                s[2 * h] = tc::ffma2v(make_float2(d[0], d[1]), fmul2(before, ksc[2 * h][k]), s[2 * h]);
+                s[2 * h + 1] = tc::ffma2v(make_float2(d[2], d[3]), fmul2(before, ksc[2 * h + 1][k]), s[2 * h + 1]);
             }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[r] = fmul2(s[r], make_float2(c0, c1));
+            s[r] = fmul2(s[r], after);
             if (!whole && g + 8 * (r & 1) >= nl[r >> 1]) s[r] = make_float2(-INFINITY, -INFINITY);
         }
         const float t0 = fmaxf(fmaxf(s[0].x, s[1].x), fmaxf(s[2].x, s[3].x));

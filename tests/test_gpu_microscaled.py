@@ -408,6 +408,39 @@ def test_attention_weights_have_the_accuracy_of_32_bits(hd, bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("key_exp,query_exp", [(110, -108), (-118, 119), (118, -118), (60, -58), (0, 0)])
+@pytest.mark.parametrize("grp", [1, 5])
+def test_attention_over_the_range_of_keys_and_queries(grp, key_exp, query_exp, bits):
+    """Ordinary scores from keys and queries near both ends of the range."""
+    g = gen(grp + bits + key_exp)
+    c = fk.MxKvCache(20, 16, 2, 64, bits=bits, device=DEV)
+    k = (torch.randn(c.slots, 128, generator=g, device=DEV).double() * 2.0 ** key_exp).to(BF16)
+    v = torch.randn(c.slots, 128, generator=g, device=DEV).to(BF16)
+    q = (torch.randn(2, grp * 128, generator=g, device=DEV).double() * 2.0 ** query_exp).to(BF16)
+    fk.kv_cache_write(c, k, v, torch.arange(c.slots, device=DEV))
+    t = torch.randperm(20, generator=g, device=DEV).to(torch.int32).view(1, 20).expand(2, 20)
+    got = fk.attention_1q_cached(q, c, t, i32([c.slots, 77]))
+    assert torch.isfinite(got).all()
+    check_attend(got, q, c, k, v, t, [c.slots, 77], bits)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_attention_scores_up_to_the_range_of_32_bits(bits):
+    """Queries of ones over keys of 2^110: products of a key pass 2^117, the largest score takes all."""
+    g = gen(bits)
+    c = fk.MxKvCache(8, 16, 1, 128, bits=bits, device=DEV)
+    k = (torch.randn(c.slots, 128, generator=g, device=DEV).double() * 2.0 ** 110).to(BF16)
+    v = torch.randn(c.slots, 128, generator=g, device=DEV).to(BF16)
+    fk.kv_cache_write(c, k, v, torch.arange(c.slots, device=DEV))
+    got = host(fk.attention_1q_cached(torch.ones(1, 128, device=DEV, dtype=BF16), c, i32([list(range(8))]), i32([c.slots])))
+    score = np.sort(mxo.values(host(k), bits).sum(1))
+    best = mxo.values(host(k), bits).sum(1).argmax()
+    assert score[-1] - score[-2] > 1e-3 * score[-1]           # far more than fp32 sums are off by
+    want = mxo.values(host(v), bits)[best]                    # 8-bit and 4-bit values are bf16 values
+    assert np.array_equal(got[0], want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("order", ["first", "last", "each group"])
 def test_attention_huge_values_without_weight(order, bits):
     """Values 2^90 times the others at keys whose weight is nothing beside the others': they must not
