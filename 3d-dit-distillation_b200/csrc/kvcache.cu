@@ -237,7 +237,7 @@ struct AttnArgs {
     int splits;                              // key ranges of a sequence
     int cluster;                             // CTAs of a cluster: 1, or all splits of a sequence and head
     float scale_log2;
-    float* ws;                               // [batch, heads, splits, 2 + hd] when not in a cluster
+    float* ws;                               // [batch, heads, splits, 2 + hd] when not in a cluster: m, l, mean
 };
 
 // a sequence's length, held inside its table row
@@ -249,6 +249,15 @@ __device__ __forceinline__ int64_t length_of(const AttnArgs& a, int page_size, i
     }
     return n;
 }
+
+// the output from the largest score, the sum of the weights and the weighted mean: zeros where there were no
+// keys, and not a number where there were and none had any weight (all scores -inf)
+__device__ __forceinline__ float joined_output(float m, float l, float mean) {
+    return m == -INFINITY ? 0.f : l == 0.f ? __uint_as_float(0x7fffffffu) : mean;
+}
+
+// 1 / a sum of weights, within 2 ulp (the sums stay far below 2^126, where this division ends); 0 for none
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : __fdividef(1.f, l); }
 
 // a float of shared memory at the same place in CTA `rank` of the cluster
 __device__ __forceinline__ float load_cluster(uint32_t addr, int rank) {
@@ -634,7 +643,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         m0 = fmaxf(m0, -FLT_MAX);
         m1 = fmaxf(m1, -FLT_MAX);
     }
-    // join the warps through shared memory
+    // join the warps through shared memory.  What is joined, here and over the splits, is the largest score m,
+    // the sum l of the weights and the weighted mean of the values: sums of values could pass fp32's range
+    // where their mean does not
 #pragma unroll
     for (int w = 4; w < 32; w <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, w);
@@ -651,6 +662,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         x[2] = m1;
         x[3] = l1;
     }
+    const float n0 = inverse(l0), n1 = inverse(l1);
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
         const float u0 = __uint_as_float(max((uint32_t)(254 - field(k, 0)) << 23, 0x00400000u));      // 1 / inv
@@ -658,7 +670,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const float* x = o[2 * k + e];
-            float2 v0 = make_float2(x[0] * u0, x[2] * u0), v1 = make_float2(x[1] * u1, x[3] * u1);
+            float2 v0 = make_float2(x[0] * n0 * u0, x[2] * n0 * u0), v1 = make_float2(x[1] * n1 * u1, x[3] * n1 * u1);
             if (PARTS == 1) {                               // the weights' second parts, of columns 4 to 7
                 v0 = tc::fadd2(v0, make_float2(__shfl_down_sync(0xffffffffu, v0.x, 2), __shfl_down_sync(0xffffffffu, v0.y, 2)));
                 v1 = tc::fadd2(v1, make_float2(__shfl_down_sync(0xffffffffu, v1.x, 2), __shfl_down_sync(0xffffffffu, v1.y, 2)));
@@ -675,17 +687,19 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
         float mm = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml[(w * kQ + j) * 2]);
-        float acc = 0.f, ll = 0.f;
+        float acc = 0.f, ll = 0.f, f[kWarps];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float mw = ml[(w * kQ + j) * 2];
-            const float f = mw == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : exp2f(mw - mm);
-            acc += so[(w * kQ + j) * HD + e] * f;
-            ll += ml[(w * kQ + j) * 2 + 1] * f;
+            f[w] = mw == -INFINITY ? 0.f : exp2f(mw - mm) * ml[(w * kQ + j) * 2 + 1];
+            ll += f[w];
         }
+        const float share = inverse(ll);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) acc = fmaf(so[(w * kQ + j) * HD + e], f[w] * share, acc);
         const int h = kh * a.group + q0 + j;
         if (a.splits == 1) {
-            a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(mm == -INFINITY ? 0.f : acc / ll);
+            a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(joined_output(mm, ll, acc));
         } else if (a.cluster == 1) {
             float* x = a.ws + (((int64_t)b * a.heads + h) * a.splits + split) * (2 + HD);
             x[2 + e] = acc;
@@ -703,22 +717,26 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(Cache c, AttnArgs a
     }
     if (a.cluster == 1) return;
     // the splits of a sequence and head are the CTAs of this cluster: each joins its part of the
-    // outputs through distributed shared memory
+    // outputs through distributed shared memory.  A warp's 32 outputs are of one query: lane r has the
+    // weight of rank r
     tc::cluster_sync();
     const uint32_t so_at = tc::smem_u32(so), joined_at = tc::smem_u32(joined);
     for (int i = split * kWarps * 32 + threadIdx.x; i < nq * HD; i += a.cluster * kWarps * 32) {
         const int j = i / HD;
-        float mm = -INFINITY;
-        for (int r = 0; r < a.cluster; ++r) mm = fmaxf(mm, load_cluster(joined_at + j * 8, r));
-        float acc = 0.f, ll = 0.f;
-#pragma unroll 4
-        for (int r = 0; r < a.cluster; ++r) {
-            const float mr = load_cluster(joined_at + j * 8, r);
-            const float f = mr == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : exp2f(mr - mm);
-            acc = fmaf(load_cluster(so_at + i * 4, r), f, acc);
-            ll = fmaf(load_cluster(joined_at + j * 8 + 4, r), f, ll);
+        const float mr = lane < a.cluster ? load_cluster(joined_at + j * 8, lane) : -INFINITY;
+        const float lr = lane < a.cluster ? load_cluster(joined_at + j * 8 + 4, lane) : 0.f;
+        const float mm = warp_max(mr);
+        const float f = mr == -INFINITY ? 0.f : exp2f(mr - mm) * lr;
+        const float ll = warp_sum(f), share = f * inverse(ll);
+        float acc = 0.f;
+        for (int r0 = 0; r0 < a.cluster; r0 += 8) {
+            float x[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] = r0 + r < a.cluster ? load_cluster(so_at + i * 4, r0 + r) : 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) acc = fmaf(x[r], __shfl_sync(0xffffffffu, share, r0 + r), acc);
         }
-        a.out[b * a.ldo + (int64_t)(kh * a.group + q0) * HD + i] = f2bf(mm == -INFINITY ? 0.f : acc / ll);
+        a.out[b * a.ldo + (int64_t)(kh * a.group + q0) * HD + i] = f2bf(joined_output(mm, ll, acc));
     }
     tc::cluster_sync();                                     // no CTA leaves while another reads its memory
 }
@@ -741,9 +759,9 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
     float ll = 0.f;
     for (int i = e; i < a.splits; i += HD) {
         const float mi = base[i * (2 + HD)];
-        const float f = mi == -INFINITY ? (mm == -INFINITY ? 1.f : 0.f) : exp2f(mi - mm);
+        const float f = mi == -INFINITY ? 0.f : exp2f(mi - mm) * base[i * (2 + HD) + 1];
         weight[i] = f;
-        ll += base[i * (2 + HD) + 1] * f;
+        ll += f;
     }
     ll = warp_sum(ll);
     if (lane == 0) red[1][warp] = ll;
@@ -751,10 +769,11 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
     ll = 0.f;
 #pragma unroll
     for (int w = 0; w < HD / 32; ++w) ll += red[1][w];
+    const float share = inverse(ll);
     float acc = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < a.splits; ++i) acc = fmaf(base[i * (2 + HD) + 2 + e], weight[i], acc);
-    a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(mm == -INFINITY ? 0.f : acc / ll);
+    for (int i = 0; i < a.splits; ++i) acc = fmaf(base[i * (2 + HD) + 2 + e], weight[i] * share, acc);
+    a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(joined_output(mm, ll, acc));
 }
 
 // How the keys of a sequence are split: two rounds of the CTAs that fit the GPU (3 of 4 warps on each

@@ -441,6 +441,24 @@ def test_attention_scores_up_to_the_range_of_32_bits(bits):
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("batch,n,grp", [(1, 4, 1), (1, 200, 5), (1, 4101, 1), (1, 20000, 2), (300, 130, 1)])
+def test_attention_sums_of_values_past_the_range(batch, n, grp, bits):
+    """Values of one sign near bf16's largest: their sum over the keys is out of range, their mean is not.
+    One warp, one CTA, a cluster and the second kernel join the parts."""
+    g = gen(n + grp + bits)
+    c = fk.MxKvCache(-(-n // 16), 16, 2, 64, bits=bits, device=DEV)
+    k = torch.randn(c.slots, 128, generator=g, device=DEV).to(BF16)
+    v = ((torch.rand(c.slots, 128, generator=g, device=DEV) * 0.7 + 1).double() * 2.0 ** 126).to(BF16)
+    fk.kv_cache_write(c, k, v, torch.arange(c.slots, device=DEV))
+    q = torch.randn(batch, grp * 128, generator=g, device=DEV).to(BF16)
+    t = torch.randperm(c.pages, generator=g, device=DEV).to(torch.int32)[None].expand(batch, c.pages)
+    got = fk.attention_1q_cached(q, c, t, i32([n] * batch))
+    assert torch.isfinite(got).all()
+    for b in {0, batch - 1}:
+        check_attend(got[b:b + 1], q[b:b + 1], c, k, v, t[b:b + 1], [n], bits)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("order", ["first", "last", "each group"])
 def test_attention_huge_values_without_weight(order, bits):
     """Values 2^90 times the others at keys whose weight is nothing beside the others': they must not
