@@ -532,7 +532,8 @@ int linear_codes(const void* a_codes, const void* a_scales, const void* w_codes,
 // of a 128-row block), a lane one block of 32 of each at a time; the first blocks are on their way
 // before the CTA quantises the rows of a into shared memory.  Products of half a block are summed in
 // f16 pairs, exactly: 8 products of at most 36, all multiples of 1/4, stay below 2^11 quarters.  Across
-// blocks the sums are fp32.  Against quantising and the MMA kernel (for 7680 x 1536): one row 5.1
+// blocks the sums are fp32; a block's sum takes the smaller of its two scales first, so that the
+// product overflows only where the result does.  Against quantising and the MMA kernel (for 7680 x 1536): one row 5.1
 // against 8.2 us, two 6.4; four 11.7, but with a launch less, which the host takes 5 us for; 8 rows
 // would take 18.5.
 constexpr int kFewRows = 4;
@@ -555,6 +556,18 @@ struct FewArgs {
 
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 pair(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+
+// the smaller and the larger of two scales; a NaN stays one
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 // MT: rows of a, rounded up to a power of two (the rows past m are zeros)
 template <int T, int MT>
@@ -659,7 +672,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) few_rows_kernel(const __grid_c
                         h1 = __hfma2(w[r][8 + j], x[8 + j], h1);
                     }
                     const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                    acc[r][i] = fmaf(((f0.x + f0.y) + (f1.x + f1.y)) * sc[r], e, acc[r][i]);
+                    acc[r][i] = fmaf(((f0.x + f0.y) + (f1.x + f1.y)) * min_nan(sc[r], e), max_nan(sc[r], e), acc[r][i]);
                 }
             }
         }

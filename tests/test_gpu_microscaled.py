@@ -181,6 +181,17 @@ def test_linear_over_the_range_of_scales(m):
     assert (fk.linear_mxfp4(x, fk.quantize_mxfp4(w)).float() == want).all()
 
 
+@pytest.mark.parametrize("x_exp,w_exp", [(-120, 124), (124, -120), (-60, 62), (3, -3)])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 130])
+def test_linear_of_large_weights_and_small_rows(m, x_exp, w_exp):
+    """Ordinary products of operands near both ends of the range, and blocks of zeros between them."""
+    g = gen(m + x_exp)
+    x = (torch.randn(m, 160, generator=g, device=DEV).double() * 2.0 ** x_exp).to(BF16)
+    w = (torch.randn(72, 160, generator=g, device=DEV).double() * 2.0 ** w_exp).to(BF16)
+    x[:, 32:64], w[:, 64:96] = 0, 0
+    check_linear(fk.linear_mxfp4(x, fk.quantize_mxfp4(w)), x, w, None)
+
+
 # ----------------------------------------------------------------------------- cache
 
 def filled(g, pages, page, heads, hd, bits):
