@@ -132,7 +132,7 @@ class OptimizedLatDitRunner:
         # CUDA-graph replay of the sampler (per voxel count, context length and schedule)
         self.cuda_graph = bool(cuda_graph)
         # block linears held and multiplied in 4-bit microscaled form (approximate; off by default)
-        self.mxfp4_linears = tuple(mxfp4_linears)
+        self.mxfp4_linears = tuple(dict.fromkeys(mxfp4_linears))      # a name given twice counts once
         if self.mxfp4_linears and (a.dim % 32 or a.ffn_dim % 32):
             raise ValueError(f"mxfp4_linears: widths {a.dim} and {a.ffn_dim} must be multiples of 32")
         self._graphs: "OrderedDict[tuple, _SampleGraph]" = OrderedDict()

@@ -788,3 +788,15 @@ def test_runner_in_four_bits_captured():
     graphed = [r.sample_with_context(vox, ctx, noise=xt, cuda_graph=True) for _ in range(2)]
     assert torch.isfinite(eager).all()
     assert torch.equal(graphed[0], graphed[1]) and torch.equal(graphed[0], eager)
+
+
+def test_runner_takes_a_name_given_twice_once():
+    from vdit.fast_flow import OptimizedLatDitRunner
+    from vdit.fast_sampler import SolverConfig
+    model, vox, ctx, xt = _model(depth=2, cond_depth=1)
+    once, twice = (OptimizedLatDitRunner(model, SolverConfig(), device=torch.device(DEV), mxfp4_linears=names)
+                   for names in (("ffn0", "ffn1"), ["ffn0", "ffn1", "ffn0"]))
+    assert twice.mxfp4_linears == ("ffn0", "ffn1")
+    for a, b in zip(once.blocks, twice.blocks):
+        for n in ("ffn0", "ffn1"):
+            assert torch.equal(a[n].codes, b[n].codes) and torch.equal(a[n].scales, b[n].scales)
