@@ -649,6 +649,57 @@ def test_captured_and_on_another_stream():
             assert all(torch.equal(a, b) for a, b in zip(got, w))
 
 
+def test_workspaces_of_calls_in_flight_at_once():
+    """Two captured graphs replayed on two streams beside eager calls on a third, at sizes where the attention's
+    splits and the linear's quantised rows go through workspaces: none sees another's."""
+    from vdit import microscaled
+    heads, hd, page, pages, d = 2, 128, 64, 320, 256
+    assert microscaled._attend_workspace(2, 2 * heads, heads, hd, pages, page) > 0     # a second kernel joins
+    assert microscaled._dense_workspace(300, d) > 0                                    # rows quantised, then multiplied
+
+    def state(seed):
+        g = gen(seed)
+        c, _, _ = filled(g, pages, page, heads, hd, 8)
+        return {"c": c, "q": torch.randn(2, 2 * d, generator=g, device=DEV).to(BF16),
+                "t": torch.stack([torch.randperm(pages, generator=g, device=DEV) for _ in range(2)]).to(torch.int32),
+                "n": i32([pages * page - seed, 9000 + seed]), "x": torch.randn(300, d, generator=g, device=DEV).to(BF16),
+                "w": fk.quantize_mxfp4(torch.randn(512, d, generator=g, device=DEV).to(BF16))}
+
+    def step(s):
+        out = []
+        for _ in range(6):
+            out.append(fk.attention_1q_cached(s["q"], s["c"], s["t"], s["n"]))
+            out.append(fk.linear_mxfp4(s["x"], s["w"]))
+            out.append(fk.linear_mxfp4(out[-1][:, d:], s["w"]))
+        return out
+
+    states = [state(1), state(2), state(3)]
+    want = [[t.clone() for t in step(s)[:3]] for s in states]
+    torch.cuda.synchronize()
+    graphs = []
+    for s in states[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(s)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(20):
+        for _, out in graphs:
+            for t in out:
+                t.zero_()
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        got = [graphs[0][1], graphs[1][1], None]
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i][0].replay()
+        with torch.cuda.stream(streams[2]):
+            got[2] = step(states[2])
+        torch.cuda.synchronize()
+        for out, w in zip(got, want):
+            assert all(torch.equal(t, w[i % 3]) for i, t in enumerate(out))
+
+
 @pytest.mark.parametrize("rows", [3, 700, 9000])
 def test_each_call_waits_for_the_one_before(rows):
     """Every call reads what the call before it wrote (a kernel, a copy or another stream's kernel), in
