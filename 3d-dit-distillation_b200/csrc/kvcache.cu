@@ -776,12 +776,16 @@ __global__ void __launch_bounds__(HD) combine_kernel(AttnArgs a) {
     a.out[b * a.ldo + (int64_t)h * HD + e] = f2bf(joined_output(mm, ll, acc));
 }
 
-// How the keys of a sequence are split: two rounds of the CTAs that fit the GPU (3 of 4 warps on each
-// of 148 SMs) but no fewer than 128 keys of the longest sequence, one group a warp; four rounds,
-// for an even end, where a split then still has 1024.  Where up to 16 splits that all run at once have
-// no more than 2048 keys each, they are a cluster, which joins them itself (one launch, no workspace);
-// otherwise their states go through the workspace to a second kernel (16 sequences of up to 32768
-// keys: 200 us when this was chosen, 183 now; in clusters of 2 or 8 272 and 233).
+// How the keys of a sequence are split: two rounds of 3 CTAs on each of 148 SMs but no fewer than 128 keys
+// of the longest sequence, one group a warp; four rounds, for an even end, where a split then still has
+// 1024.  3 CTAs are what an SM holds of 128 channels and of 64 in 8 bits; of 96 channels it holds 4, of 64
+// in 4 bits 5, of 32 6 or 8, so there a round is a part of one.  Up to 16 splits with no more than 2048 keys
+// each, and no more than 4 CTAs an SM in all, are a cluster, which joins them itself (one launch, no
+// workspace); otherwise their states go through the workspace to a second kernel (16 sequences of up to
+// 32768 keys: 200 us when this was chosen, 191 now; in clusters of 2 or 8 272 and 233 then).
+// The longest sequence is the table's width: the lengths are on the GPU.  A table far wider than its
+// sequences is planned for as if it were full (16 sequences of up to 300 keys, 12 x 128: 10.4 us in a table of
+// 300 or 4096 keys, 21.8 in one of 32768).
 // Queries of a CTA, at most: 4 with both parts of their weights in one MMA, 8 with two.  16 sequences over 8
 // key heads of 96 channels, 8 bits: 4 queries a key head (up to 20000 keys) 76 us with 4, 81 with 8; 5 queries
 // (up to 16000 keys) 105 with 4 (two CTAs read the same keys), 73 with 8.
@@ -821,9 +825,9 @@ int launch_attend(const Cache& c, const AttnArgs& a, int batch, cudaStream_t s) 
         return VDIT_ERR_LAUNCH;
     }
     const dim3 grid(a.splits, c.heads * ((a.group + SLOTS - 1) / SLOTS), batch);
-    // Set up while the kernel before it ends.  In a stream of calls 16 ragged sequences take 18.9 us instead of
-    // 20.5 and one of 4101 keys 12.6 either way; replayed in a graph, where launches are close already,
-    // the one sequence takes 12.4 instead of 11.9.
+    // Set up while the kernel before it ends.  When this was chosen, 16 ragged sequences took 18.9 us in a stream of
+    // calls instead of 20.5 and one of 4101 keys 12.6 either way; replayed in a graph, where launches are
+    // close already, the one sequence took 12.4 instead of 11.9 (12.2 now).
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -457,9 +457,13 @@ int launch(const Call& c) {
 }
 
 // Tile for an [m, n] output: of the pairs' widths and the single CTA's 64 columns the one with
-// the least estimated time, rounds of tiles over the GPU x the time of a tile.  Measured at
-// k = 1536, us on 256 / 192 / 128 / 64 columns: 128 x 1536 7.9 / 6.9 / 6.7 / 5.5, 2048 x 1536
-// 8.7 / 8.2 / 9.6 / 10.0, 4101 x 1536 12.3 / 12.0 / 12.4 / 16.7, 4101 x 7680 27.9 / 31.7 / 38.0 / 60.2.
+// the least estimated time, rounds of tiles over the GPU x the time of a tile (whose ratios hardly depend
+// on k).  Product alone, us on 256 / 192 / 128 / 64 columns, * the one picked:
+//   k = 1536   128 x 1536 7.5 / 7.0 / 6.3 / 5.1*, 2048 x 1536 9.0 / 8.5* / 9.3 / 10.0,
+//              4101 x 1536 11.8 / 11.2* / 11.6 / 16.0, 4101 x 7680 27.9* / 31.5 / 36.7 / 59.9
+//   k = 3840   128 x 1536 10.5 / 10.2 / 9.4 / 8.2*, 2048 x 1536 12.0 / 11.4* / 14.6 / 17.3,
+//              4632 x 1536 18.5* / 21.5 / 24.3 / 31.6, 16384 x 1536 42.4 / 44.0* / 59.2 / 101
+//   k = 320    4101 x 7680 18.9* / 21.8 / 20.6 / 30.1, 4632 x 1536 9.2* / 9.8 / 9.1 / 9.9
 int pick_tile(int64_t m, int n, int sms) {
     const int widths[4] = {256, 192, 128, 64};
     const double cost[4] = {1.0, 0.8, 0.6, 0.35};
@@ -533,9 +537,13 @@ int linear_codes(const void* a_codes, const void* a_scales, const void* w_codes,
 // before the CTA quantises the rows of a into shared memory.  Products of half a block are summed in
 // f16 pairs, exactly: 8 products of at most 36, all multiples of 1/4, stay below 2^11 quarters.  Across
 // blocks the sums are fp32; a block's sum takes the smaller of its two scales first, so that the
-// product overflows only where the result does.  Against quantising and the MMA kernel (for 7680 x 1536): one row 5.1
-// against 8.2 us, two 6.4; four 11.7, but with a launch less, which the host takes 5 us for; 8 rows
-// would take 18.5.
+// product overflows only where the result does.
+// Graph replays with weights beyond L2, no bias, us for 1 / 2 / 3 / 4 rows here and for 5 by the quantiser and
+// the MMA kernel: 7680 x 1536 5.8 / 7.0 / 12.2 / 12.5 and 7.6, 1536 x 1536 3.7 / 4.5 / 6.0 / 6.2 and 5.4, 16384 x 4096
+// 15 / 20 / 39 / 40 and 21.  Calls one after another from Python, where each launch is host time: 7680 x 1536 8.8 / 8.9 /
+// 12.3 / 12.3 and 12.5, 1536 x 1536 8.8 / 9.0 / 8.9 / 8.9 and 12.6, 16384 x 4096 16 / 21 / 41 / 41 and 21.  So 3 and 4 rows
+// gain a launch for small weights and lose time for large ones; the limit knows no n because the
+// workspace's size does not.
 constexpr int kFewRows = 4;
 constexpr int kFewWarps = 8;
 constexpr int64_t kFewElements = 65536;      // of a, rows rounded up: 136 KB of shared memory

@@ -392,7 +392,9 @@ int vdit_kv_cache_read(const vdit_kv_cache* cache, const int64_t* slots, int64_t
  * length are not read (ld_table 0: every sequence has the same pages).  No keys give zeros.  q bf16
  * [batch, ldq] and out bf16 [batch, ldo] hold heads * head_dim channels a row; query head h reads key
  * head h / (heads / cache->heads).  A page outside the cache is left out and a length outside
- * [0, max_pages * page_size] is clipped to it, both recorded in the device error word.  Partial
+ * [0, max_pages * page_size] is clipped to it, both recorded in the device error word.  Scores, weights
+ * and sums have fp32's accuracy and range.  The keys are split by max_pages, not by the lengths: give
+ * no more columns of the table than the longest sequence may need.  Partial
  * states of split keys may go to the caller's workspace (of vdit_attention_1q_cached_workspace_bytes
  * bytes, 16-byte aligned; may be 0). */
 size_t vdit_attention_1q_cached_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t head_dim,
