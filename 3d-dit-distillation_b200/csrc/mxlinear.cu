@@ -538,19 +538,22 @@ int linear_codes(const void* a_codes, const void* a_scales, const void* w_codes,
 // f16 pairs, exactly: 8 products of at most 36, all multiples of 1/4, stay below 2^11 quarters.  Across
 // blocks the sums are fp32; a block's sum takes the smaller of its two scales first, so that the
 // product overflows only where the result does.
-// Graph replays with weights beyond L2, no bias, us for 1 / 2 / 3 / 4 rows here and for 5 by the quantiser and
-// the MMA kernel: 7680 x 1536 5.8 / 7.0 / 12.2 / 12.5 and 7.6, 1536 x 1536 3.7 / 4.5 / 6.0 / 6.2 and 5.4, 16384 x 4096
-// 15 / 20 / 39 / 40 and 21.  Calls one after another from Python, where each launch is host time: 7680 x 1536 8.8 / 8.9 /
-// 12.3 / 12.3 and 12.5, 1536 x 1536 8.8 / 9.0 / 8.9 / 8.9 and 12.6, 16384 x 4096 16 / 21 / 41 / 41 and 21.  So 3 and 4 rows
-// gain a launch for small weights and lose time for large ones; the limit knows no n because the
-// workspace's size does not.
+// One and two rows, graph replays with weights beyond L2, no bias, here / by the quantiser and the MMA kernel, us:
+// 7680 x 1536 5.8, 7.0 / 7.6, 1536 x 1536 3.7, 4.5 / 5.4, 16384 x 4096 15, 20 / 21.  Three and four rows are
+// the slower ones on the GPU, but a launch less is host time where calls follow one another from Python;
+// graph (calls), here / there: 1536 x 640 4.3 (9) / 4.5 (13), 1536 x 2048 6.2 (9) / 6.1 (13), 7680 x 1536 12.4 (14) /
+// 7.7 (13), 1536 x 2560 8.5 (10) / 6.9 (13), 1536 x 3840 11 (12) / 9.0 (13), 16384 x 4096 39 (41) / 21 (21).  So they
+// come here up to k = 2048; the rule knows no n because the workspace's size does not.
 constexpr int kFewRows = 4;
+constexpr int kFewWide = 2048;
 constexpr int kFewWarps = 8;
 constexpr int64_t kFewElements = 65536;      // of a, rows rounded up: 136 KB of shared memory
 constexpr int kFewSmem = (int)(kFewElements * 2 + kFewElements / kBlock * 4);
 
 int few_rounded(int64_t m) { return m <= 2 ? (int)m : 4; }
-bool few_rows(int64_t m, int k) { return m <= kFewRows && (int64_t)few_rounded(m) * k <= kFewElements; }
+bool few_rows(int64_t m, int k) {
+    return m <= kFewRows && (m <= 2 || k <= kFewWide) && (int64_t)few_rounded(m) * k <= kFewElements;
+}
 
 struct FewArgs {
     const void* x;

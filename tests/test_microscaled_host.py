@@ -132,6 +132,16 @@ def test_c_entry_points_check_before_any_launch():
     assert lib.vdit_attention_1q_cached(*a) == -5
 
 
+def test_which_rows_are_quantised_on_the_way():
+    """No workspace for one and two rows of up to 65536 elements in all, and for three and four of up to 2048."""
+    need = _lib.load().vdit_linear_mxfp4_dense_workspace_bytes
+    for m, k, none in ((1, 65536, True), (1, 65568, False), (2, 32768, True), (2, 32800, False), (3, 2048, True),
+                       (4, 2048, True), (3, 2080, False), (4, 2080, False), (5, 32, False)):
+        assert (need(m, k) == 0) == none, (m, k)
+        if not none:
+            assert need(m, k) == m * k // 2 + -(-m // 128) * -(-k // 128) * 512
+
+
 @pytest.mark.parametrize("pages,page,heads,hd,bits", [(3, 16, 5, 96, 4), (7, 16, 2, 32, 8), (2, 1024, 3, 128, 8),
                                                        (70000, 128, 12, 128, 8)])
 def test_cache_addresses_stay_inside_and_apart(pages, page, heads, hd, bits):
