@@ -369,12 +369,10 @@ __global__ void __launch_bounds__(threads_of<EPI>(), 1) gemm_kernel(const __grid
     __syncthreads();
     // an abort is the pair's: the peer need not wait its own limit out
     if (threadIdx.x == 0 && *abort_flag) store_cluster(mapa_shared(smem_u32(&sm.abort_flag), rank ^ 1), 1);
-    __syncwarp();
     cluster_sync();    // no CTA leaves while its peer's MMAs or arrivals may still touch it
     if (*abort_flag) {
         // a wait ran out: the loads and MMAs still in flight end before either CTA does
         if (threadIdx.x == 0) store_cluster(mapa_shared(smem_u32(&sm.peer_fills), rank ^ 1), fills);
-        __syncwarp();
         cluster_sync();
         if (leader && warp == 1) {
             volatile int gave_up = 0;

@@ -323,7 +323,10 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t cta) {
     return r;
 }
 
+// The barrier's aligned form is for whole warps: one of which a single lane has just run a role (a producer's
+// loop) is brought together first, or it could arrive in parts.
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 

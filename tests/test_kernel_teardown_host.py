@@ -37,3 +37,10 @@ def test_a_cta_of_a_pair_leaves_after_every_commit_on_its_stages(name):
     """The tensor core delivers a commit to both CTAs by itself; each waits for the last one of every stage."""
     assert re.search(r"for \(int j = max\(0, it - (NST|STAGES)\); ok && j < it; \+\+j\)\s*"
                      r"ok = mbar_wait\(smem_u32\(&sm\.empty\[", FILES[name])
+
+
+def test_cluster_barriers_are_for_whole_warps():
+    """The aligned form of the cluster barrier stands in one place, behind a warp barrier."""
+    header = re.sub(r"//.*", "", (CSRC / "tc.cuh").read_text())
+    assert re.search(r"void cluster_sync\(\) \{\s*__syncwarp\(\);\s*asm volatile\(\s*\"barrier\.cluster\.arrive", header)
+    assert len(re.findall(r"barrier\.cluster", header)) == 2 and not any("barrier.cluster" in t for t in FILES.values())
