@@ -118,6 +118,8 @@ class Phases:
     def check(self):
         code = self.error_word() if self.error_word is not None else 0
         if code:
+            if code < 0:
+                raise SystemExit(f"bench: the device error word cannot be read (code {code}) after phase '{self.name}'")
             raise SystemExit(f"bench: device error word {code:#x} ({code.to_bytes(4, 'big').strip(bytes(1))!r}) after "
                              f"phase '{self.name}'")
 

@@ -25,3 +25,8 @@ def test_phases_that_end_leave_the_process_alone():
 def test_an_error_word_is_named_with_its_phase():
     r = run("p = bench.Phases(60.0, error_word=lambda: 0x474D)\np('warm-up')\np('timed steps')")
     assert r.returncode == 1 and "0x474d (b'GM') after phase 'warm-up'" in r.stderr and "timed steps" not in r.stderr
+
+
+def test_an_error_word_that_cannot_be_read_is_an_error():
+    r = run("p = bench.Phases(60.0, error_word=lambda: -3)\np('warm-up')\np.done()")
+    assert r.returncode == 1 and "cannot be read (code -3) after phase 'warm-up'" in r.stderr
