@@ -708,6 +708,7 @@ class OptimizedLatDitRunner:
                                  should_eval_uncond(i, n_guided, sc.cfg_stride, sc.cfg_cache_mode,
                                                     sc.eval_uncond_steps))
             neg = self._negative_stream() if (eval_neg and self.overlap_branches) else main
+            self._get_time_gates(tl[i])                   # made here, if they are new, before the streams part
             if neg is not main:
                 neg.wait_stream(main)                     # x_t of this step
                 xt.record_stream(neg)
